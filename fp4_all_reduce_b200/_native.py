@@ -28,6 +28,7 @@ REC_PAYLOAD = 3472
 MODE_FUSED, MODE_XPORT, MODE_COMPUTE = 0, 1, 2
 ALGO_AUTO, ALGO_ONESHOT, ALGO_TWOSHOT = -1, 0, 1
 IN_BF16, IN_NVFP4, IN_PUSHED = 0, 1, 2
+ACT_SILU, ACT_GELU, ACT_GELU_TANH = 0, 1, 2
 EPI_NONE, EPI_NORM_BF16, EPI_NORM_NVFP4, EPI_NORM_MXFP8 = 0, 1, 2, 3
 
 ERROR_NAMES = {0: "ok", 1: "bad argument", 2: "unsupported combination", 3: "CUDA error", 4: "context poisoned"}
@@ -139,6 +140,14 @@ def cuda() -> C.CDLL:
     lib.fp4ar_gemm_reset.restype = C.c_int
     lib.fp4ar_gemm_workspace.argtypes = [vp]
     lib.fp4ar_gemm_workspace.restype = vp
+    lib.fp4ar_gated_linear.argtypes = [vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp]
+    lib.fp4ar_gated_linear.restype = C.c_int
+    lib.fp4ar_gated_backward.argtypes = [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp]
+    lib.fp4ar_gated_backward.restype = C.c_int
+    lib.fp4ar_adapters_workspace.argtypes = [C.c_int, C.c_int, C.c_int]
+    lib.fp4ar_adapters_workspace.restype = C.c_size_t
+    lib.fp4ar_linear_adapters.argtypes = [vp, vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp]
+    lib.fp4ar_linear_adapters.restype = C.c_int
     for name in ("fp4ar_create", "fp4ar_create_emulated", "fp4ar_launch", "fp4ar_status", "fp4ar_set_timeout_ms",
                  "fp4ar_reset", "fp4ar_destroy", "fp4ar_get_push_view", "fp4ar_ctas_per_rank", "fp4ar_encode",
                  "fp4ar_encode_static", "fp4ar_decode_sum", "fp4ar_reduce_reencode", "fp4ar_add_rmsnorm",

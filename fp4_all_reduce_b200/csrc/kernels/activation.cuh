@@ -1,0 +1,43 @@
+// The gates of the gated feed-forward block and their derivatives, in FP32.
+//
+//   silu        a = g s,  a' = s (1 + g (1 - s)),  s = 1 / (1 + e^-g)
+//   gelu        a = g P,  a' = P + g p,  P = erfc(-g / sqrt 2) / 2 (no cancellation for negative g),  p = e^(-g^2/2) / sqrt(2 pi)
+//   gelu_tanh   a = g s,  a' = s + g s (1 - s) w',  s = sigmoid(w),  w = 2 sqrt(2/pi) (g + 0.044715 g^3): (1 + tanh(w/2)) / 2 = s
+//
+// __expf and __fdividef are off by a few 2^-22 here, against the 2^-9 of the BF16 rounding that follows.  Far from zero the
+// exponential overflows to infinity and s becomes an exact 0.
+#pragma once
+#include <cuda_runtime.h>
+#include "../include/fp4ar_layer.h"
+
+namespace fp4ar {
+
+__device__ __forceinline__ float sigmoid_f32(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
+__device__ __forceinline__ float gelu_tanh_arg(float g) { return 1.5957691216f * fmaf(0.044715f * g * g, g, g); }
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float g) {
+  if constexpr (ACT == FP4AR_ACT_SILU) return g * sigmoid_f32(g);
+  else if constexpr (ACT == FP4AR_ACT_GELU) return 0.5f * g * erfcf(-0.70710678119f * g);
+  else return g * sigmoid_f32(gelu_tanh_arg(g));
+}
+
+// value and derivative
+template <int ACT>
+__device__ __forceinline__ void act_both(float g, float& value, float& slope) {
+  if constexpr (ACT == FP4AR_ACT_SILU) {
+    const float s = sigmoid_f32(g);
+    value = g * s;
+    slope = s * fmaf(g, 1.0f - s, 1.0f);
+  } else if constexpr (ACT == FP4AR_ACT_GELU) {
+    const float P = 0.5f * erfcf(-0.70710678119f * g);
+    value = g * P;
+    slope = fmaf(g, 0.39894228040f * __expf(-0.5f * g * g), P);
+  } else {
+    const float s = sigmoid_f32(gelu_tanh_arg(g)), t = s * (1.0f - s);
+    value = g * s;
+    slope = t == 0.0f ? s : fmaf(g * t, 1.5957691216f * fmaf(0.134145f, g * g, 1.0f), s);      // t = 0: g^2 may be infinite
+  }
+}
+
+}  // namespace fp4ar

@@ -1,0 +1,114 @@
+// Gated projections of the feed-forward block: h = a(x Wg^T) * (x Wu^T) in one kernel (layer_gemm.cuh), and their gradients.
+//
+// Backward: dpre = (dh u a'(g), dh a(g)) elementwise from the projections that the forward pass kept in BF16, then two products
+// dx = dpre W and dW = dpre^T x.  dpre is rounded to BF16 once, as the tensor cores take it.
+#include "layer_gemm.cuh"
+
+namespace fp4ar {
+namespace layer {
+
+// One thread has eight neighbouring columns of a row: three 16-byte loads, two 16-byte stores; five bytes of traffic per two of
+// dh, so it is bound by memory.
+template <int ACT>
+__global__ void gated_grad_kernel(const uint4* __restrict__ dh, const uint4* __restrict__ pre, uint4* __restrict__ dpre, int M, int f8) {
+  pdl_wait_prior_grids();
+  pdl_release_dependents();
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= f8) return;
+  for (long row = blockIdx.y; row < M; row += gridDim.y) {
+    const uint4 d = dh[row * f8 + c], g = pre[row * 2 * f8 + c], u = pre[(row * 2 + 1) * f8 + c];
+    const uint32_t dw[4] = {d.x, d.y, d.z, d.w}, gw[4] = {g.x, g.y, g.z, g.w}, uw[4] = {u.x, u.y, u.z, u.w};
+    uint32_t og[4], ou[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float a0, s0, a1, s1;
+      act_both<ACT>(bf16_lo(gw[i]), a0, s0);
+      act_both<ACT>(bf16_hi(gw[i]), a1, s1);
+      const float d0 = bf16_lo(dw[i]), d1 = bf16_hi(dw[i]);
+      og[i] = pack_bf16(d0 * bf16_lo(uw[i]) * s0, d1 * bf16_hi(uw[i]) * s1);
+      ou[i] = pack_bf16(d0 * a0, d1 * a1);
+    }
+    dpre[row * 2 * f8 + c] = make_uint4(og[0], og[1], og[2], og[3]);
+    dpre[(row * 2 + 1) * f8 + c] = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+  }
+}
+
+static int launch_grad(const void* dh, const void* pre, void* dpre, int M, int F, int act, cudaStream_t stream) {
+  const int f8 = F / 8;
+  const int block = f8 < 256 ? (f8 + 31) / 32 * 32 : 256, gx = (f8 + block - 1) / block;
+  int gy = device_sm_count() * 16 * (256 / block) / gx;        // enough warps for every SM, then a walk over the rows
+  gy = gy < 1 ? 1 : gy > M ? M : gy;
+  if (gy > 65535) gy = 65535;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(gx, gy);
+  cfg.blockDim = dim3(block);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto kernel = act == FP4AR_ACT_SILU ? gated_grad_kernel<FP4AR_ACT_SILU>
+                : act == FP4AR_ACT_GELU ? gated_grad_kernel<FP4AR_ACT_GELU> : gated_grad_kernel<FP4AR_ACT_GELU_TANH>;
+  if (cudaLaunchKernelEx(&cfg, kernel, (const uint4*)dh, (const uint4*)pre, (uint4*)dpre, M, f8) != cudaSuccess) return cuda_fail();
+  return cuda_check_launch();
+}
+
+static bool shape_ok(int M, int F, int K, int act) {
+  return M >= 0 && F >= 8 && K >= 8 && F % 8 == 0 && K % 8 == 0 && act >= FP4AR_ACT_SILU && act <= FP4AR_ACT_GELU_TANH &&
+         extents_ok((long long)M + 256, 2LL * F + 256) && extents_ok(K, 0);
+}
+
+}  // namespace layer
+}  // namespace fp4ar
+
+using namespace fp4ar;
+using namespace fp4ar::layer;
+
+extern "C" int fp4ar_gated_linear(const void* x, const void* wt, int M, int F, int K, int act, void* h, void* pre, fp4ar_stream stream) {
+  if (!shape_ok(M, F, K, act)) return FP4AR_ERR_ARGUMENT;
+  if (M == 0) return FP4AR_OK;
+  if (!x || !wt || !h || !aligned16(x, wt, h, pre)) return FP4AR_ERR_ARGUMENT;
+  Maps maps;
+  memset(&maps, 0, sizeof(maps));
+  if (!map_2d(&maps.a, x, M, K, 128) || !map_2d(&maps.b, wt, 2L * F, K, 128) || !map_2d(&maps.out, h, M, F, 32) ||
+      (pre && !map_pre(&maps.pre, pre, M, F)))
+    return FP4AR_ERR_UNSUPPORTED;
+  Params p;
+  memset(&p, 0, sizeof(p));
+  p.M = M; p.N = F; p.kblocks = (K + 63) / 64; p.act = act; p.want_pre = pre != nullptr;
+  return launch_pair_gemm<kGated>(maps, p, (cudaStream_t)stream);
+}
+
+extern "C" int fp4ar_gated_backward(const void* dh, const void* pre, const void* x, const void* wt, int M, int F, int K, int act,
+                                    void* dpre, void* dx, void* dwt, fp4ar_stream stream_) {
+  if (!shape_ok(M, F, K, act)) return FP4AR_ERR_ARGUMENT;
+  const cudaStream_t stream = (cudaStream_t)stream_;
+  if (M == 0) {
+    if (dwt && cudaMemsetAsync(dwt, 0, (size_t)2 * F * K * 2, stream) != cudaSuccess) return cuda_fail();
+    return FP4AR_OK;
+  }
+  if (!dh || !pre || !dpre || (dx && !wt) || (dwt && !x) || !aligned16(dh, pre, dpre) || !aligned16(x, wt, dx, dwt)) return FP4AR_ERR_ARGUMENT;
+  int rc = launch_grad(dh, pre, dpre, M, F, act, stream);
+  if (rc != FP4AR_OK) return rc;
+  Params p;
+  if (dx) {
+    Maps maps;
+    memset(&maps, 0, sizeof(maps));
+    memset(&p, 0, sizeof(p));
+    if (!map_2d(&maps.a, dpre, M, 2L * F, 128) || !map_2d(&maps.b, wt, 2L * F, K, 64) || !map_2d(&maps.out, dx, M, K, 32)) return FP4AR_ERR_UNSUPPORTED;
+    p.M = M; p.N = K; p.kblocks = (2 * F + 63) / 64;
+    rc = launch_pair_gemm<kInput>(maps, p, stream);
+    if (rc != FP4AR_OK) return rc;
+  }
+  if (dwt) {
+    Maps maps;
+    memset(&maps, 0, sizeof(maps));
+    memset(&p, 0, sizeof(p));
+    if (!map_2d(&maps.a, dpre, M, 2L * F, 64) || !map_2d(&maps.b, x, M, K, 64) || !map_2d(&maps.out, dwt, 2L * F, K, 32)) return FP4AR_ERR_UNSUPPORTED;
+    p.M = 2 * F; p.N = K; p.kblocks = (M + 63) / 64;
+    rc = launch_pair_gemm<kWeight>(maps, p, stream);
+  }
+  return rc;
+}

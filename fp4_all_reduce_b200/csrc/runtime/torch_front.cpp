@@ -24,6 +24,7 @@
 #include <torch/library.h>
 #include "../include/fp4ar.h"
 #include "../include/fp4ar_gemm.h"
+#include "../include/fp4ar_layer.h"
 
 namespace {
 
@@ -42,6 +43,10 @@ struct Api {
   decltype(&fp4ar_reduce_reencode) reduce_reencode;
   decltype(&fp4ar_add_rmsnorm) add_rmsnorm;
   decltype(&fp4ar_gemm_nvfp4) gemm;
+  decltype(&fp4ar_gated_linear) gated_linear;
+  decltype(&fp4ar_gated_backward) gated_backward;
+  decltype(&fp4ar_adapters_workspace) adapters_workspace;
+  decltype(&fp4ar_linear_adapters) linear_adapters;
 };
 Api api{};
 PyObject* check_rc = nullptr;      // _native.check(rc, what): raises the Python error of a return code
@@ -228,12 +233,131 @@ std::tuple<Tensor, Tensor> op_gemm(const Tensor& x, const Tensor& wt, double gs,
   return {std::move(q), std::move(acc)};
 }
 
+// ---- gated projections, adapters ----
+// A contiguous tensor of this shape that the tensor maps can describe.
+void require_matrix(const Tensor& t, at::ScalarType dtype, at::IntArrayRef shape, c10::Device dev, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == dtype, name, " must be ", dtype_name(dtype), ", got ", dtype_name(t.scalar_type()));
+  TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape, ", got ", shape_text(t));
+  TORCH_CHECK_VALUE(t.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA tensor");
+  require_on(t, dev, name);
+  TORCH_CHECK_VALUE((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 || t.numel() == 0, name, " must start on a 16-byte boundary");
+}
+void require_apart(const Tensor& out, const Tensor& in, const char* name) {
+  const char *a = (const char*)out.data_ptr(), *b = (const char*)in.data_ptr();
+  TORCH_CHECK_VALUE(out.numel() == 0 || in.numel() == 0 || a + out.nbytes() <= b || b + in.nbytes() <= a, "out must not overlap ", name);
+}
+// Rows and columns as the C interface takes them: 32-bit, with room for a tile.
+void require_size(int64_t n, const char* name) { TORCH_CHECK_VALUE(n <= 0x7fff0000, name, " is too large: ", n); }
+
+struct GatedShape {
+  int64_t M, K, F;
+  GatedShape(const Tensor& x, const Tensor& wt, int64_t act) {
+    TORCH_CHECK_VALUE(x.dim() == 2, "x must have shape [rows, K], got ", shape_text(x));
+    TORCH_CHECK_VALUE(wt.dim() == 2 && wt.size(1) == x.size(1), "wt must have shape [2 F, ", x.size(1), "], got ", shape_text(wt));
+    M = x.size(0); K = x.size(1); F = wt.size(0) / 2;
+    TORCH_CHECK_VALUE(K >= 8 && K % 8 == 0, "K must be a positive multiple of 8, got ", K);
+    TORCH_CHECK_VALUE(F >= 8 && wt.size(0) % 16 == 0, "wt must have 2 F rows, F a positive multiple of 8, got ", wt.size(0), " rows");
+    TORCH_CHECK_VALUE(act >= FP4AR_ACT_SILU && act <= FP4AR_ACT_GELU_TANH, "activation must be 0 (silu), 1 (gelu) or 2 (gelu_tanh)");
+    require_size(M, "rows"); require_size(K, "K"); require_size(2 * F, "2 F");
+    require_matrix(x, at::kBFloat16, {M, K}, x.device(), "x");
+    require_matrix(wt, at::kBFloat16, {2 * F, K}, x.device(), "wt");
+  }
+};
+
+std::tuple<Tensor, Tensor> op_gated_linear(const Tensor& x, const Tensor& wt, int64_t act, bool want_pre, Tensor out) {
+  const GatedShape s(x, wt, act);
+  const c10::Device dev = x.device();
+  if (out.defined()) {
+    require_matrix(out, at::kBFloat16, {s.M, s.F}, dev, "out");
+    require_apart(out, x, "x");
+    require_apart(out, wt, "wt");
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  if (!out.defined()) out = new_empty({s.M, s.F}, at::kBFloat16, dev);
+  Tensor pre;
+  if (want_pre) pre = new_empty({s.M, 2 * s.F}, at::kBFloat16, dev);
+  ok(api.gated_linear(x.data_ptr(), wt.data_ptr(), (int)s.M, (int)s.F, (int)s.K, (int)act, out.mutable_data_ptr(),
+                      want_pre ? pre.mutable_data_ptr() : nullptr, stream_of(dev)), "fp4ar_gated_linear");
+  return {std::move(out), std::move(pre)};
+}
+
+std::tuple<Tensor, Tensor> op_gated_backward(const Tensor& dh, const Tensor& pre, const Tensor& x, const Tensor& wt, int64_t act, bool need_dx,
+                                             bool need_dw) {
+  const GatedShape s(x, wt, act);
+  const c10::Device dev = x.device();
+  require_matrix(dh, at::kBFloat16, {s.M, s.F}, dev, "dh");
+  require_matrix(pre, at::kBFloat16, {s.M, 2 * s.F}, dev, "pre");
+  const c10::cuda::CUDAGuard guard(dev);
+  Tensor dx, dw;
+  if (!need_dx && !need_dw) return {dx, dw};
+  if (need_dx) dx = new_empty({s.M, s.K}, at::kBFloat16, dev);
+  if (need_dw) dw = new_empty({2 * s.F, s.K}, at::kBFloat16, dev);
+  Tensor dpre = new_empty({s.M, 2 * s.F}, at::kBFloat16, dev);
+  ok(api.gated_backward(dh.data_ptr(), pre.data_ptr(), x.data_ptr(), wt.data_ptr(), (int)s.M, (int)s.F, (int)s.K, (int)act,
+                        dpre.mutable_data_ptr(), need_dx ? dx.mutable_data_ptr() : nullptr, need_dw ? dw.mutable_data_ptr() : nullptr,
+                        stream_of(dev)), "fp4ar_gated_backward");
+  return {std::move(dx), std::move(dw)};
+}
+
+Tensor op_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, const Tensor& a, const Tensor& b, const Tensor& scales, Tensor out) {
+  TORCH_CHECK_VALUE(x.dim() == 2, "x must have shape [rows, K], got ", shape_text(x));
+  TORCH_CHECK_VALUE(wt.dim() == 2 && wt.size(1) == x.size(1), "wt must have shape [N, ", x.size(1), "], got ", shape_text(wt));
+  const int64_t M = x.size(0), K = x.size(1), Nn = wt.size(0);
+  TORCH_CHECK_VALUE(K >= 8 && K % 8 == 0 && Nn >= 8 && Nn % 8 == 0, "K and N must be positive multiples of 8, got ", K, " and ", Nn);
+  TORCH_CHECK_VALUE(a.dim() == 3 && a.size(2) == K, "a must have shape [adapters, R, ", K, "], got ", shape_text(a));
+  const int64_t n = a.size(0), R = a.size(1);
+  TORCH_CHECK_VALUE(n >= 1, "a must hold at least one adapter");
+  TORCH_CHECK_VALUE(R >= 8 && R % 8 == 0 && R <= 128, "the rank must be a multiple of 8 up to 128 (pad with zeros), got ", R);
+  require_size(M, "rows"); require_size(K, "K"); require_size(n * Nn, "adapters x N");
+  const c10::Device dev = x.device();
+  require_matrix(x, at::kBFloat16, {M, K}, dev, "x");
+  require_matrix(wt, at::kBFloat16, {Nn, K}, dev, "wt");
+  require_matrix(a, at::kBFloat16, {n, R, K}, dev, "a");
+  require_matrix(b, at::kBFloat16, {n, Nn, R}, dev, "b");
+  require(ids, at::kInt, -1, "ids");
+  TORCH_CHECK_VALUE(ids.dim() == 1 && ids.size(0) == M, "ids must have shape (", M, ",), got ", shape_text(ids));
+  require_on(ids, dev, "ids");
+  if (scales.defined()) {
+    require(scales, at::kFloat, -1, "scales");
+    TORCH_CHECK_VALUE(scales.dim() == 1 && scales.size(0) == n, "scales must have shape (", n, ",), got ", shape_text(scales));
+    require_on(scales, dev, "scales");
+  }
+  if (out.defined()) {
+    require_matrix(out, at::kBFloat16, {M, Nn}, dev, "out");
+    require_apart(out, x, "x"); require_apart(out, wt, "wt"); require_apart(out, ids, "ids");
+    require_apart(out, a, "a"); require_apart(out, b, "b");
+    if (scales.defined()) require_apart(out, scales, "scales");
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  if (!out.defined()) out = new_empty({M, Nn}, at::kBFloat16, dev);
+  Tensor ws = new_empty({(int64_t)api.adapters_workspace((int)M, (int)R, (int)n)}, at::kByte, dev);
+  ok(api.linear_adapters(x.data_ptr(), wt.data_ptr(), (const int*)ids.data_ptr(), a.data_ptr(), b.data_ptr(),
+                         scales.defined() ? (const float*)scales.data_ptr() : nullptr, (int)M, (int)Nn, (int)K, (int)R, (int)n,
+                         ws.mutable_data_ptr(), out.mutable_data_ptr(), stream_of(dev)), "fp4ar_linear_adapters");
+  return out;
+}
+
 // ---- torch.ops.fp4ar.* (the schemas are defined in ops/allreduce.py) ----
 Tensor lib_decode_sum(const std::vector<Tensor>& q, const std::vector<Tensor>& rs) { return op_decode_sum(q, rs, {}, false); }
 Tensor lib_add_rms_norm(const Tensor& x, Tensor& residual, const Tensor& weight, double eps, double weight_bias) {
   return std::get<0>(op_norm(x, residual, weight, eps, weight_bias, FP4AR_EPI_NORM_BF16, 1.0, true, Tensor()));
 }
 Tensor lib_linear(const Tensor& x, const Tensor& wt, double gs) { return std::get<0>(op_gemm(x, wt, gs, false, Tensor())); }
+
+Tensor lib_gated_linear(const Tensor& x, const Tensor& wt, int64_t act) { return std::get<0>(op_gated_linear(x, wt, act, false, Tensor())); }
+std::tuple<Tensor, Tensor> lib_gated_linear_pre(const Tensor& x, const Tensor& wt, int64_t act) { return op_gated_linear(x, wt, act, true, Tensor()); }
+std::tuple<Tensor, Tensor> lib_gated_linear_backward(const Tensor& dh, const Tensor& pre, const Tensor& x, const Tensor& wt, int64_t act, bool need_dx,
+                                                     bool need_dw) {
+  auto r = op_gated_backward(dh, pre, x, wt, act, need_dx, need_dw);
+  const auto none = [&](Tensor& t) { if (!t.defined()) t = new_empty({0}, at::kBFloat16, x.device()); };
+  none(std::get<0>(r));
+  none(std::get<1>(r));
+  return r;
+}
+Tensor lib_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, const Tensor& a, const Tensor& b, const std::optional<Tensor>& scales) {
+  return op_linear_adapters(x, wt, ids, a, b, scales ? *scales : Tensor(), Tensor());
+}
 
 // ---- Python entry points: positional arguments only, the wrappers fill in the defaults ----
 const Tensor& tensor_arg(PyObject* o, const char* name) {
@@ -355,6 +479,49 @@ PyObject* py_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   auto r = [&] { NoGil g; return op_gemm(x, wt, gs, acc, std::move(out)); }();
   if (!acc) return THPVariable_Wrap(std::move(std::get<0>(r)));
   return wrap2(std::move(std::get<0>(r)), std::move(std::get<1>(r)));
+  END_HANDLE_TH_ERRORS
+}
+PyObject* wrap_or_none(Tensor t) {
+  if (t.defined()) return THPVariable_Wrap(std::move(t));
+  Py_RETURN_NONE;
+}
+PyObject* wrap2_or_none(std::tuple<Tensor, Tensor> r) {
+  THPObjectPtr t(PyTuple_New(2));
+  if (!t) throw python_error();
+  PyTuple_SET_ITEM(t.get(), 0, wrap_or_none(std::move(std::get<0>(r))));
+  PyTuple_SET_ITEM(t.get(), 1, wrap_or_none(std::move(std::get<1>(r))));
+  return t.release();
+}
+// (x, wt, activation, want_pre, out or None): (h, pre or None)
+PyObject* py_gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 5);
+  const Tensor &x = tensor_arg(a[0], "x"), &wt = tensor_arg(a[1], "wt");
+  const int64_t act = int_arg(a[2]);
+  const bool pre = bool_arg(a[3]);
+  Tensor out = a[4] == Py_None ? Tensor() : tensor_arg(a[4], "out");
+  return wrap2_or_none([&] { NoGil g; return op_gated_linear(x, wt, act, pre, std::move(out)); }());
+  END_HANDLE_TH_ERRORS
+}
+// (dh, pre, x, wt, activation, need_dx, need_dw): (dx or None, dwt or None)
+PyObject* py_gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 7);
+  const Tensor &dh = tensor_arg(a[0], "dh"), &pre = tensor_arg(a[1], "pre"), &x = tensor_arg(a[2], "x"), &wt = tensor_arg(a[3], "wt");
+  const int64_t act = int_arg(a[4]);
+  const bool dx = bool_arg(a[5]), dw = bool_arg(a[6]);
+  return wrap2_or_none([&] { NoGil g; return op_gated_backward(dh, pre, x, wt, act, dx, dw); }());
+  END_HANDLE_TH_ERRORS
+}
+// (x, wt, ids, a, b, scales or None, out or None)
+PyObject* py_linear_adapters(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 7);
+  const Tensor &x = tensor_arg(p[0], "x"), &wt = tensor_arg(p[1], "wt"), &ids = tensor_arg(p[2], "ids"), &a = tensor_arg(p[3], "a"),
+               &b = tensor_arg(p[4], "b");
+  const Tensor scales = p[5] == Py_None ? Tensor() : tensor_arg(p[5], "scales");
+  Tensor out = p[6] == Py_None ? Tensor() : tensor_arg(p[6], "out");
+  return THPVariable_Wrap([&] { NoGil g; return op_linear_adapters(x, wt, ids, a, b, scales, std::move(out)); }());
   END_HANDLE_TH_ERRORS
 }
 
@@ -509,7 +676,9 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const bool all = bind(lib, "fp4ar_launch", api.launch) && bind(lib, "fp4ar_last_cuda_error", api.last_error) &&
                    bind(lib, "fp4ar_encode", api.encode) && bind(lib, "fp4ar_encode_static", api.encode_static) &&
                    bind(lib, "fp4ar_decode_sum", api.decode_sum) && bind(lib, "fp4ar_reduce_reencode", api.reduce_reencode) &&
-                   bind(lib, "fp4ar_add_rmsnorm", api.add_rmsnorm) && bind(lib, "fp4ar_gemm_nvfp4", api.gemm);
+                   bind(lib, "fp4ar_add_rmsnorm", api.add_rmsnorm) && bind(lib, "fp4ar_gemm_nvfp4", api.gemm) &&
+                   bind(lib, "fp4ar_gated_linear", api.gated_linear) && bind(lib, "fp4ar_gated_backward", api.gated_backward) &&
+                   bind(lib, "fp4ar_adapters_workspace", api.adapters_workspace) && bind(lib, "fp4ar_linear_adapters", api.linear_adapters);
   if (!all) throw std::runtime_error(std::string(path) + " lacks a function of the C interface");
   Py_INCREF(a[1]);
   Py_XSETREF(check_rc, a[1]);
@@ -519,7 +688,8 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FP4AR_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FP4AR_METHOD(bind), FP4AR_METHOD(encode), FP4AR_METHOD(encode_static), FP4AR_METHOD(decode_sum),
-                         FP4AR_METHOD(reduce_reencode), FP4AR_METHOD(add_rmsnorm), FP4AR_METHOD(gemm), {nullptr, nullptr, 0, nullptr}};
+                         FP4AR_METHOD(reduce_reencode), FP4AR_METHOD(add_rmsnorm), FP4AR_METHOD(gemm), FP4AR_METHOD(gated_linear), FP4AR_METHOD(gated_backward),
+                         FP4AR_METHOD(linear_adapters), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fp4ar_front", nullptr, -1, methods};
 
 }  // namespace
@@ -530,6 +700,10 @@ TORCH_LIBRARY_IMPL(fp4ar, CUDA, m) {
   m.impl("decode_sum", lib_decode_sum);
   m.impl("add_rms_norm", lib_add_rms_norm);
   m.impl("linear_nvfp4", lib_linear);
+  m.impl("gated_linear", lib_gated_linear);
+  m.impl("gated_linear_pre", lib_gated_linear_pre);
+  m.impl("gated_linear_backward", lib_gated_linear_backward);
+  m.impl("linear_adapters", lib_linear_adapters);
 }
 
 PyMODINIT_FUNC PyInit__fp4ar_front() {

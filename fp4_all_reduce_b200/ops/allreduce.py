@@ -12,6 +12,8 @@ implementations, and recordable in CUDA graphs (a launch has no host-side per-ca
     y = torch.ops.fp4ar.all_reduce_add_rms_norm_nvfp4(xq, gs, residual, weight, 1e-6, 1.0, ctx_id)
     y = torch.ops.fp4ar.linear_all_reduce_add_rms_norm(x, wt, gs, residual, weight, 1e-6, 1.0, ctx_id)   # row-parallel linear:
                                                            # tcgen05 GEMM pushing NVFP4 partials into the peers + AllReduce + norm
+    h = torch.ops.fp4ar.gated_linear(x, wt, 0)             # gated projections (ops/ffn.py); differentiable in x and wt
+    y = torch.ops.fp4ar.linear_adapters(h, wt, ids, a, b, scales)     # row-parallel linear with adapters (ops/adapters.py)
 
 This is the op surface the reference project only plans (docs/INTEGRATION.md:18-23).
 """
@@ -58,6 +60,10 @@ _lib.define("add_rms_norm(Tensor x, Tensor(a!) residual, Tensor weight, float ep
 _lib.define("linear_nvfp4(Tensor x, Tensor wt, float gs) -> Tensor")
 _lib.define("linear_all_reduce_add_rms_norm(Tensor x, Tensor wt, float[] gs, Tensor(a!) residual, Tensor weight, float eps, "
             "float weight_bias, int ctx) -> Tensor")
+_lib.define("gated_linear(Tensor x, Tensor wt, int activation) -> Tensor")
+_lib.define("gated_linear_pre(Tensor x, Tensor wt, int activation) -> (Tensor, Tensor)")
+_lib.define("gated_linear_backward(Tensor dh, Tensor pre, Tensor x, Tensor wt, int activation, bool need_dx, bool need_dw) -> (Tensor, Tensor)")
+_lib.define("linear_adapters(Tensor x, Tensor wt, Tensor ids, Tensor a, Tensor b, Tensor? scales) -> Tensor")
 
 
 def _all_reduce(x, ctx):
@@ -107,7 +113,8 @@ except (RuntimeError, OSError, ImportError) as _e:          # not built here: th
     def _missing(*_args, _why=str(_e)):
         raise RuntimeError(_why)
 
-    for _name in ("encode", "encode_static", "decode_sum", "add_rms_norm", "linear_nvfp4"):
+    for _name in ("encode", "encode_static", "decode_sum", "add_rms_norm", "linear_nvfp4", "gated_linear", "gated_linear_pre",
+                  "gated_linear_backward", "linear_adapters"):
         _lib.impl(_name, _missing, "CUDA")
 
 
@@ -170,3 +177,40 @@ def _(x, wt, gs, residual, weight, eps, weight_bias, ctx):
 @torch.library.register_fake("fp4ar::add_rms_norm")
 def _(x, residual, weight, eps, weight_bias):
     return torch.empty_like(x)
+
+
+@torch.library.register_fake("fp4ar::gated_linear")
+def _(x, wt, activation):
+    return x.new_empty((x.shape[0], wt.shape[0] // 2))
+
+
+@torch.library.register_fake("fp4ar::gated_linear_pre")
+def _(x, wt, activation):
+    return x.new_empty((x.shape[0], wt.shape[0] // 2)), x.new_empty((x.shape[0], wt.shape[0]))
+
+
+@torch.library.register_fake("fp4ar::gated_linear_backward")
+def _(dh, pre, x, wt, activation, need_dx, need_dw):
+    return x.new_empty(x.shape if need_dx else (0,)), x.new_empty(wt.shape if need_dw else (0,))
+
+
+@torch.library.register_fake("fp4ar::linear_adapters")
+def _(x, wt, ids, a, b, scales):
+    return x.new_empty((x.shape[0], wt.shape[0]))
+
+
+def _gated_setup(ctx, inputs, output):
+    x, wt, ctx.activation = inputs
+    ctx.save_for_backward(x, wt)
+
+
+def _gated_grad(ctx, dh):
+    # the op returns h alone, so its backward pass computes the projections again; `ops.ffn.gated_linear` keeps them
+    x, wt = ctx.saved_tensors
+    need_dx, need_dw = ctx.needs_input_grad[:2]
+    pre = torch.ops.fp4ar.gated_linear_pre(x, wt, ctx.activation)[1]
+    dx, dw = torch.ops.fp4ar.gated_linear_backward(dh.contiguous(), pre, x, wt, ctx.activation, need_dx, need_dw)
+    return dx if need_dx else None, dw if need_dw else None, None
+
+
+torch.library.register_autograd("fp4ar::gated_linear", _gated_grad, setup_context=_gated_setup)
