@@ -18,7 +18,7 @@ extern "C" {
 enum { FP4AR_ACT_SILU = 0, FP4AR_ACT_GELU = 1, FP4AR_ACT_GELU_TANH = 2 };
 
 /* h[M,F] = a(x Wg^T) * (x Wu^T), x [M,K], wt [2F,K]: the F gate rows, then the F up rows.  K and F are multiples of 8.
- * pre: optional [M,2F], the two projections in BF16 (what the backward pass takes); h does not go through that rounding. */
+ * pre: optional [M,2F] FP32, the two projections (what the backward pass takes). */
 int fp4ar_gated_linear(const void* x, const void* wt, int M, int F, int K, int act, void* h, void* pre, fp4ar_stream stream);
 
 /* Gradients of h for dh [M,F].  dpre [M,2F] BF16 is written: (dh up a'(gate), dh a(gate)); then
@@ -33,6 +33,11 @@ int fp4ar_gated_backward(const void* dh, const void* pre, const void* x, const v
 size_t fp4ar_adapters_workspace(int M, int R, int adapters);
 int fp4ar_linear_adapters(const void* x, const void* wt, const int* ids, const void* a, const void* b, const float* scales, int M, int N,
                           int K, int R, int adapters, void* workspace, void* y, fp4ar_stream stream);
+
+/* How these products share their work (host only): `tiles` output tiles of `kblocks` K blocks over `units` CTA pairs.  *used: units that
+ * work.  With `segments` the work of `unit` as (tile, first K block, K blocks, kind: 0 whole, 1 leaves a partial, 2 finishes the
+ * tile, units that leave partials for it); returns the number of segments (also beyond max_segments), -1 for bad arguments. */
+int fp4ar_layer_plan(int tiles, int kblocks, int units, int unit, int* used, int* segments, int max_segments);
 
 #ifdef __cplusplus
 }

@@ -143,4 +143,31 @@ __device__ __forceinline__ void gemm_settle(uint64_t* bar, uint32_t parity) {
   while (!mbar_test(bar, parity) && global_timer_ns() - t0 < 10000000ull) {}
 }
 
+// Bounded wait until *flag == want (acquire); false when it gave up or the CTA is aborting.
+__device__ __forceinline__ uint32_t ld_acquire_gpu(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_release_gpu(uint32_t* p, uint32_t v) {
+  asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+__device__ __forceinline__ bool gemm_flag_wait(const uint32_t* flag, uint32_t want, const GemmWait& w, uint32_t what) {
+  if (ld_acquire_gpu(flag) == want) return true;
+  const unsigned long long t0 = global_timer_ns();
+  uint32_t n = 0;
+  while (ld_acquire_gpu(flag) != want) {
+    if ((++n & 63u) == 0u) {
+      if (*w.abort_flag) return false;
+      if (global_timer_ns() - t0 > w.limit_ns) {
+        *w.abort_flag = 1u;
+        if (atomicCAS(&w.status->code, 0u, (uint32_t)kStatusLoadTimeout) == 0u) { w.status->detail = 16u + what; w.status->cta = blockIdx.x; }
+        atomicAdd(&w.status->count, 1u);
+        return false;
+      }
+    }
+  }
+  return true;
+}
+
 }  // namespace fp4ar

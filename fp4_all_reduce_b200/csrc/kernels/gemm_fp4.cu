@@ -47,6 +47,7 @@
 #include "../include/fp4ar_gemm.h"
 #include "../include/fp4ar_tensor.cuh"
 #include "host_util.h"
+#include "split_space.h"
 #include "tensor_map.h"
 
 namespace fp4ar {
@@ -112,33 +113,6 @@ __device__ __forceinline__ void tile_coords(int t, int m_tiles, int n_tiles, int
   const int width = min(kPanel, n_tiles - panel * kPanel);
   const int m = within / width, n = panel * kPanel + within % width;
   m0 = m * kBM * G; n0 = n * BN;
-}
-
-// Bounded wait until *flag == want (acquire); false when it gave up or the CTA is aborting.
-__device__ __forceinline__ uint32_t ld_acquire_gpu(const uint32_t* p) {
-  uint32_t v;
-  asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_release_gpu(uint32_t* p, uint32_t v) {
-  asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
-__device__ __forceinline__ bool gemm_flag_wait(const uint32_t* flag, uint32_t want, const GemmWait& w, uint32_t what) {
-  if (ld_acquire_gpu(flag) == want) return true;
-  const unsigned long long t0 = global_timer_ns();
-  uint32_t n = 0;
-  while (ld_acquire_gpu(flag) != want) {
-    if ((++n & 63u) == 0u) {
-      if (*w.abort_flag) return false;
-      if (global_timer_ns() - t0 > w.limit_ns) {
-        *w.abort_flag = 1u;
-        if (atomicCAS(&w.status->code, 0u, (uint32_t)kStatusLoadTimeout) == 0u) { w.status->detail = 16u + what; w.status->cta = blockIdx.x; }
-        atomicAdd(&w.status->count, 1u);
-        return false;
-      }
-    }
-  }
-  return true;
 }
 
 // The work of one CTA as a list of segments (tile, K blocks [lo, lo + count), rotation), the same list in all three roles.
@@ -659,7 +633,8 @@ StatusWords* gemm_status_word() {
   return p;
 }
 
-// Workspaces of the stream-K split: one slot of 128 x 256 floats and four flags per SM (19 MB on a B200).  A flag says that
+// Workspaces of the stream-K split: one slot of 128 x 256 floats and eight flags per SM (19 MB on a B200; this kernel takes four flags
+// per CTA, layer_gemm.cuh eight).  A flag says that
 // a partial is there, not whose it is, so two launches that may run at the same time never share a workspace:
 //   - the launches of a stream follow one another and share one (streams are told apart by their id, which is never used
 //     again).  The first kSpaces streams of a device have their own; the launches of all later ones take turns on one
@@ -682,7 +657,7 @@ constexpr int kSpaces = 8;
 static StreamKPool* const g_stream_k = new StreamKPool[64];      // never destroyed: a graph may be released while the process ends
 static std::mutex g_stream_k_mu;
 static size_t stream_k_partial_bytes() { return (size_t)device_sm_count() * kBM * 256 * sizeof(float); }
-static size_t stream_k_flag_bytes() { return (size_t)device_sm_count() * 4 * sizeof(uint32_t); }
+static size_t stream_k_flag_bytes() { return (size_t)device_sm_count() * kSplitFlags * sizeof(uint32_t); }
 
 // The workspace of one launch, held until the launch is enqueued.
 class StreamKLease {
@@ -776,6 +751,11 @@ class StreamKLease {
   StreamKSpace* space_ = nullptr;
   cudaEvent_t turn_ = nullptr;
 };
+
+SplitSpace::SplitSpace(cudaStream_t stream) : lease_(new StreamKLease(stream)) {}
+SplitSpace::~SplitSpace() { delete lease_; }
+float* SplitSpace::partial() const { return *lease_ ? lease_->partial() : nullptr; }
+uint32_t* SplitSpace::flags() const { return *lease_ ? lease_->flags() : nullptr; }
 
 }  // namespace fp4ar
 

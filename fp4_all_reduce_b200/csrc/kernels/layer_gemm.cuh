@@ -14,7 +14,9 @@
 //   warp 0      TMA producer
 //   warp 1      MMA issuer (even CTA), owns the 512 TMEM columns: two accumulators, so a tile's epilogue runs under the next
 //               tile's main loop
-//   warps 2-5   epilogue: tcgen05.ld, activation, BF16, a 32 x 64 slab per warp in swizzled shared memory, TMA store
+//   warps 2-9   epilogue, two per TMEM lane quarter with half of the columns each: tcgen05.ld, activation, BF16, a 32 x 64 slab per
+//               warp in swizzled shared memory, TMA store
+//   warps 10-11 kAdapt: the blocks of low-rank factors
 // Ragged sizes need no code in the main loop: tensor maps fill with zeros beyond their extents and stores are clipped.
 //
 // MN-major tiles: a box of 64 (outer index, 128 bytes, swizzled) x 64 K rows is 8 KB; a tile of 128 is two boxes.  In the
@@ -22,11 +24,13 @@
 #pragma once
 #include <atomic>
 #include <cstring>
+#include <optional>
 #include <cuda_bf16.h>
 #include "../include/fp4ar_layer.h"
 #include "../include/fp4ar_tensor.cuh"
 #include "activation.cuh"
 #include "host_util.h"
+#include "split_space.h"
 #include "tensor_map.h"
 
 namespace fp4ar {
@@ -34,13 +38,15 @@ namespace layer {
 
 enum : int { kGated = 0, kInput = 1, kWeight = 2, kAdapt = 3 };
 
-constexpr int kRowsCta = 128, kBlockK = 64, kHalf = 128, kStages = 6, kThreads = 192;
+constexpr int kRowsCta = 128, kBlockK = 64, kHalf = 128, kStages = 6;
+template <int OP> constexpr int kThreads = OP == kAdapt ? 384 : 320;
 constexpr int kOpBytes = kRowsCta * kBlockK * 2;               // 16 KB of A, 16 KB of B per CTA and stage
 constexpr int kStage = 2 * kOpBytes;
 constexpr int kSlab = 32 * 64 * 2;                             // 32 rows x 64 BF16 columns, one warp's store
-constexpr int kSlabs = 4 * 2 * kSlab;                          // two per epilogue warp
-constexpr int kSmemBytes = kStages * kStage + kSlabs + 256 + 1024;
+constexpr int kSlabs = 8 * kSlab;                              // one per epilogue warp
+constexpr int kSmemBytes = kStages * kStage + kSlabs + 512 + 1024;
 constexpr int kListStride = 260;                               // per 256-row tile: count, then up to 256 adapters (16-byte pitch)
+constexpr int kVerdicts = 16;                                  // a granted stage is six segments ahead of the MMAs at most, these two of the epilogue
 constexpr int kChunk = 32;                                     // ranks per block of low-rank factors
 
 struct Params {
@@ -48,12 +54,14 @@ struct Params {
   int kblocks;
   int act;
   bool want_pre;
+  int cut_units;            // units that share the cut tiles, 0: none are cut (see Walk)
+  float* partial;           // [CTA][8][8][128] float4
+  uint32_t* flags;          // [CTA][kSplitFlags]: 1 = that epilogue warp's part of the slot is written and not yet consumed
   // adapters
   int R, adapters;
   const int* ids;           // [M]
-  const float* v;           // [M][R] scaled x A^T, FP32
+  const __nv_bfloat16* v;   // [M][chunks of 32 ranks][64] scaled x A^T: the rounded values, then what the rounding left
   const int* lists;         // [row tiles][kListStride]
-  const unsigned char* unsafe;   // [adapters] 1: B holds infinities or NaN
   const __nv_bfloat16* b;   // [adapters][N][R]
   StatusWords* status;
   unsigned long long timeout_ns;
@@ -105,48 +113,103 @@ __host__ __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles
   n = panel * kPanelTiles + within % width;
 }
 
+// The work of a unit (CTA pair) as a list of segments (tile, K blocks [lo, lo + count)), the same list in all roles.
+//   whole tiles:  unit, unit + units, ...
+//   cut tiles:    where the tiles do not fill the units evenly, the first `cut` of them (units + remainder, or all of them where there
+//                 are fewer tiles than units) are laid out as tiles x kblocks blocks and cut into cut_units equal ranges.
+//                 Where the boundary of two ranges falls into a tile, the unit whose range ENDS there finishes the tile: it runs
+//                 the tile's LAST K blocks and adds what the units behind it (one, or several where a range is shorter than a
+//                 tile) leave in their slots.  A range that begins inside a tile runs that share first, so nobody waits for
+//                 work that waits for him, and every unit leaves one partial at most.  Sums are taken in the order of the units.
+enum : int { kWhole = 0, kProduce = 1, kFinish = 2 };
+struct Seg { int tile, lo, count, kind, others; };       // others: of kFinish, units behind this one that share the tile
+struct Walk {
+  int tiles, kblocks, units, cut_units, unit, t;
+  long long total, u, end;
+  __host__ __device__ Walk(int tiles_, int kblocks_, int unit_, int units_, int cut_units_)
+      : tiles(tiles_), kblocks(kblocks_), units(units_), cut_units(cut_units_), unit(unit_) {
+    const int cut = cut_units ? (tiles < units ? tiles : units + tiles % units) : 0;
+    total = (long long)cut * kblocks;
+    u = unit < cut_units ? total * unit / cut_units : 0;
+    end = unit < cut_units ? total * (unit + 1) / cut_units : 0;
+    t = cut + unit;
+  }
+  __host__ __device__ bool next(Seg& s) {
+    if (u < end) {
+      s.tile = (int)(u / kblocks);
+      const long long at = (long long)s.tile * kblocks;
+      const int off = (int)(u - at);
+      s.count = (int)(end - u < kblocks - off ? end - u : kblocks - off);
+      s.others = 0;
+      if (off > 0) {
+        int f = unit - 1;                              // the finisher: its range holds the tile's first block
+        while (total * f / cut_units > at) f--;
+        s.kind = kProduce;
+        s.lo = off - (int)(total * (f + 1) / cut_units - at);
+      } else if (s.count < kblocks) {
+        s.kind = kFinish;
+        s.lo = kblocks - s.count;
+        for (int f = unit + 1; total * f / cut_units < at + kblocks; f++) s.others++;
+      } else {
+        s.kind = kWhole;
+        s.lo = 0;
+      }
+      u += s.count;
+      return true;
+    }
+    if (t >= tiles) return false;
+    s.tile = t; s.lo = 0; s.count = kblocks; s.kind = kWhole; s.others = 0;
+    t += units;
+    return true;
+  }
+};
+
 // ---- Adapters.  y_i = x_i W^T + sum_r V[i][r] B_a[:, r], a = ids[i].  A 256-row tile has a list of the adapters its rows use; for
 // each of them and every 32 ranks follows one more block of the same accumulation: A is V of the rows that have this adapter and
 // zero elsewhere, as two BF16 halves (columns 0-31 the rounded value, 32-63 what the rounding left, so V counts with 16 bits), B is
-// B_a [128 columns x ranks] twice.  The producer warp writes the A block itself; W's blocks keep coming by TMA.
-// 0 x infinity would leak one request's broken adapter into the rows of others, so adapters whose B is not finite are
-// marked beforehand and left out here; the epilogue adds them to their own rows by plain dot products.
-__device__ __forceinline__ void write_low_rank_block(uint8_t* dst, const Params& p, int adapter, int chunk, int row0, int lane) {
-  const int ranks = min(kChunk, p.R - chunk * kChunk);         // a multiple of 8
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int r = i * 32 + lane, row = row0 + r;
-    const bool mine = row < p.M && p.ids[row] == adapter;
-    const float* v = p.v + (size_t)row * p.R + chunk * kChunk;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-      if (mine && 8 * j < ranks) {
-        const float4 f0 = *reinterpret_cast<const float4*>(v + 8 * j), f1 = *reinterpret_cast<const float4*>(v + 8 * j + 4);
-        const float f[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          hi[e] = pack_bf16(f[2 * e], f[2 * e + 1]);
-          const float h0 = bf16_lo(hi[e]), h1 = bf16_hi(hi[e]);
-          // what is not finite stays in the first half alone
-          lo[e] = pack_bf16(fabsf(h0) <= 3.4e38f ? f[2 * e] - h0 : 0.0f, fabsf(h1) <= 3.4e38f ? f[2 * e + 1] - h1 : 0.0f);
-        }
-      }
-      uint8_t* line = dst + r * 128;
-      sts16(line + ((j ^ (r & 7)) << 4), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-      sts16(line + (((4 + j) ^ (r & 7)) << 4), make_uint4(lo[0], lo[1], lo[2], lo[3]));
-    }
-  }
+// B_a [128 columns x ranks], used twice.  Two warps of their own fill the A blocks, while the producer goes on with the K blocks of
+// the next tile: one warp that did both took 5 us a block.
+// 0 x infinity would leak one request's broken adapter into the rows of others: those warps look through the 256 rows of B_a that a
+// tile takes (they come from L2, under the main loop) and write zeros for A and B where one value is not finite; the
+// epilogue then adds such adapters to their own rows by plain dot products.
+constexpr int kLowThreads = 64;
+__device__ __forceinline__ void low_rank_barrier() { asm volatile("barrier.cta.sync 1, 64;" ::: "memory"); }
+// ... and whether every one of the two warps' threads says yes
+__device__ __forceinline__ bool low_rank_all(bool yes) {
+  uint32_t v = yes;
+  asm volatile("{ .reg .pred p, r;\n"
+               "  setp.ne.u32 p, %0, 0;\n"
+               "  barrier.cta.red.and.pred r, 1, 64, p;\n"
+               "  selp.u32 %0, 1, 0, r; }"
+               : "+r"(v)::"memory");
+  return v != 0;
 }
 
-static __device__ __noinline__ float low_rank_dot(const float* v, const __nv_bfloat16* b, int R) {
+// Rows n0 .. n0 + 255 (below N) of B of one adapter: are all values finite?  By `lanes` lanes, each with its own answer.
+__device__ __forceinline__ bool low_rank_finite(const Params& p, int adapter, int n0, int lane, int lanes) {
+  const uint4* b = reinterpret_cast<const uint4*>(p.b + ((size_t)adapter * p.N + n0) * p.R);
+  const int n = min(256, p.N - n0) * (p.R / 8);
+  bool bad = false;
+#pragma unroll 8
+  for (int i = lane; i < n; i += lanes) {
+    const uint4 w = b[i];
+    for (uint32_t e : {w.x, w.y, w.z, w.w}) bad = bad || (e & 0x7F80u) == 0x7F80u || (e & 0x7F800000u) == 0x7F800000u;
+  }
+  return !bad;
+}
+static __device__ __noinline__ bool low_rank_unsafe(const Params& p, int adapter, int n0) { return !low_rank_finite(p, adapter, n0, 0, 1); }
+
+static __device__ __noinline__ float low_rank_dot(const __nv_bfloat16* v, const __nv_bfloat16* b, int R) {
   float s = 0.0f;
-  for (int r = 0; r < R; r++) s = fmaf(v[r], __bfloat162float(b[r]), s);
+  for (int r = 0; r < R; r++) {
+    const __nv_bfloat16* line = v + (r / kChunk) * 64 + r % kChunk;
+    s = fmaf(__bfloat162float(line[0]) + __bfloat162float(line[32]), __bfloat162float(b[r]), s);
+  }
   return s;
 }
 
 template <int OP>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads<OP>, 1)
 pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   constexpr bool kAMn = OP == kWeight, kBMn = OP == kWeight || OP == kInput;
   constexpr int kTileN = OP == kGated ? 128 : 256;             // output columns per tile
@@ -160,22 +223,26 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* settled = acc_empty + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(settled + 1);
+  uint64_t* granted = settled + 1;             // kAdapt, [kStages]: the stage is free for a block of low-rank factors
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(granted + kStages);
   volatile uint32_t* abort_flag = tmem_holder + 1;
+  volatile uint32_t* unsafe_tile = tmem_holder + 2;            // kAdapt, [kVerdicts]: 1 + the segment of which an adapter is left to the epilogue
   uint32_t issued = 0;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m_tiles = (p.M + 255) / 256, n_tiles = (p.N + kTileN - 1) / kTileN, tiles = m_tiles * n_tiles;
   const uint32_t crank = cluster_cta_rank();
   const bool leads = crank == 0u;
-  const int unit = blockIdx.x / 2, units = gridDim.x / 2;
+  Walk walk(tiles, p.kblocks, blockIdx.x / 2, gridDim.x / 2, p.cut_units);
+  Seg sg;
 
   if (threadIdx.x == 0) {
     // kAdapt: both producers announce a stage, since both may write into it themselves
-    for (int s = 0; s < kStages; s++) { mbar_init(full + s, OP == kAdapt ? 2 : 1); mbar_init(empty + s, 1); }
-    for (int a = 0; a < 2; a++) { mbar_init(acc_full + a, 1); mbar_init(acc_empty + a, 256); }
+    for (int s = 0; s < kStages; s++) { mbar_init(full + s, OP == kAdapt ? 2 : 1); mbar_init(empty + s, 1); mbar_init(granted + s, 1); }
+    for (int a = 0; a < 2; a++) { mbar_init(acc_full + a, 1); mbar_init(acc_empty + a, 16); }
     mbar_init(settled, 1);
     *abort_flag = 0u;
+    for (int i = 0; i < kVerdicts; i++) unsafe_tile[i] = 0u;
     mbar_init_fence();
     prefetch_tensormap(&maps.a);
     prefetch_tensormap(&maps.b);
@@ -193,60 +260,42 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   pdl_release_dependents();
 
   if (warp == 0) {
-    // ------------------------------------------------------------ producer (kAdapt: the whole warp)
-    if (OP == kAdapt || lane == 0) {
-      auto stage_free = [&](int s) {
-        const bool ok = gemm_wait(empty + s, ((issued / kStages) & 1u) ^ 1u, gw, 1);
-        return OP == kAdapt ? (bool)__all_sync(0xffffffffu, ok) : ok;
-      };
-      for (int t = unit; t < tiles; t += units) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      while (walk.next(sg)) {
         int tm, tn;
-        tile_at(t, m_tiles, n_tiles, tm, tn);
+        tile_at(sg.tile, m_tiles, n_tiles, tm, tn);
         const int m0 = tm * 256 + (int)crank * 128;
         const int n0 = OP == kGated ? tn * 128 + (int)crank * p.N : tn * 256 + (int)crank * 128;
-        for (int kb = 0; kb < p.kblocks; kb++, issued++) {
+        for (int kb = sg.lo; kb < sg.lo + sg.count; kb++, issued++) {
           const int s = issued % kStages;
-          if (!stage_free(s)) goto done;
-          if (lane == 0) {
-            uint8_t *sa = ring + s * kStage, *sb = sa + kOpBytes;
-            const uint32_t lead_full = cluster_addr(full + s, 0u);
-            if (leads) mbar_arrive_expect(full + s, 2 * kStage);
-            else if (OP == kAdapt) mbar_arrive_cluster(lead_full);
-            const int k0 = kb * kBlockK;
-            if constexpr (kAMn) {
-              tma_load_2d_pair(sa, &maps.a, m0, k0, lead_full);
-              tma_load_2d_pair(sa + 8192, &maps.a, m0 + 64, k0, lead_full);
-            } else {
-              tma_load_2d_pair(sa, &maps.a, k0, m0, lead_full);
-            }
-            if constexpr (kBMn) {
-              tma_load_2d_pair(sb, &maps.b, n0, k0, lead_full);
-              tma_load_2d_pair(sb + 8192, &maps.b, n0 + 64, k0, lead_full);
-            } else {
-              tma_load_2d_pair(sb, &maps.b, k0, n0, lead_full);
-            }
+          if (!gemm_wait(empty + s, ((issued / kStages) & 1u) ^ 1u, gw, 1)) goto done;
+          uint8_t *sa = ring + s * kStage, *sb = sa + kOpBytes;
+          const uint32_t lead_full = cluster_addr(full + s, 0u);
+          if (leads) mbar_arrive_expect(full + s, 2 * kStage);
+          else if (OP == kAdapt) mbar_arrive_cluster(lead_full);
+          const int k0 = kb * kBlockK;
+          if constexpr (kAMn) {
+            tma_load_2d_pair(sa, &maps.a, m0, k0, lead_full);
+            tma_load_2d_pair(sa + 8192, &maps.a, m0 + 64, k0, lead_full);
+          } else {
+            tma_load_2d_pair(sa, &maps.a, k0, m0, lead_full);
+          }
+          if constexpr (kBMn) {
+            tma_load_2d_pair(sb, &maps.b, n0, k0, lead_full);
+            tma_load_2d_pair(sb + 8192, &maps.b, n0 + 64, k0, lead_full);
+          } else {
+            tma_load_2d_pair(sb, &maps.b, k0, n0, lead_full);
           }
         }
-        if constexpr (OP == kAdapt) {
-          const int* list = p.lists + (size_t)tm * kListStride;
-          const int count = list[0], chunks = (p.R + kChunk - 1) / kChunk;
-          for (int j = 0; j < count; j++) {
-            const int adapter = list[1 + j];
-            if (p.unsafe[adapter]) continue;
-            for (int c = 0; c < chunks; c++, issued++) {
-              const int s = issued % kStages;
-              if (!stage_free(s)) goto done;
-              uint8_t *sa = ring + s * kStage, *sb = sa + kOpBytes;
-              write_low_rank_block(sa, p, adapter, c, m0, lane);
-              fence_smem_to_async();
-              __syncwarp();
-              if (lane == 0) {
-                const uint32_t lead_full = cluster_addr(full + s, 0u);
-                if (leads) mbar_arrive_expect(full + s, 2 * kOpBytes);
-                else mbar_arrive_cluster(lead_full);
-                tma_load_2d_pair(sb, &maps.low, c * kChunk, adapter * p.N + n0, lead_full);
-              }
-            }
+        if (OP == kAdapt && sg.kind != kProduce) {
+          // hand the next stages, as they come free, to the warps that fill them.  (Those cannot wait for `empty` themselves: a parity
+          // says nothing to who has not seen every round of a stage.)
+          const int blocks = p.lists[(size_t)tm * kListStride] * ((p.R + kChunk - 1) / kChunk);
+          for (int i = 0; i < blocks; i++, issued++) {
+            const int s = issued % kStages;
+            if (!gemm_wait(empty + s, ((issued / kStages) & 1u) ^ 1u, gw, 1)) goto done;
+            mbar_arrive(granted + s);
           }
         }
       }
@@ -260,12 +309,12 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         // the second wait takes what the other CTA's producer wrote, at cluster scope
         else return gemm_wait(full + s, round & 1u, gw, 3) && mbar_test_cluster(full + s, round & 1u);
       };
-      for (int t = unit; t < tiles; t += units, tile_i++) {
+      for (; walk.next(sg); tile_i++) {
         const uint32_t a = tile_i & 1u;
         if (!gemm_wait(acc_empty + a, ((tile_i >> 1) & 1u) ^ 1u, gw, 2)) goto done;
         tc_fence_after();
         const uint32_t d = tmem_base + a * 256;
-        for (int kb = 0; kb < p.kblocks; kb++, it++) {
+        for (int j = 0; j < sg.count; j++, it++) {
           const int s = it % kStages;
           if (!stage_ready(s, it / kStages)) goto done;
           tc_fence_after();
@@ -274,16 +323,15 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
           const uint64_t db = kBMn ? umma_desc_mn128(sa + kOpBytes) : umma_desc_k128(sa + kOpBytes);
 #pragma unroll
           for (int k = 0; k < kBlockK / 16; k++)          // 16 K columns are 32 bytes of a row, 16 K rows are 2 KB
-            umma_bf16_pair(d, da + (uint64_t)(kAMn ? 128 * k : 2 * k), db + (uint64_t)(kBMn ? 128 * k : 2 * k), kIdesc, (kb | k) != 0 ? 1u : 0u);
+            umma_bf16_pair(d, da + (uint64_t)(kAMn ? 128 * k : 2 * k), db + (uint64_t)(kBMn ? 128 * k : 2 * k), kIdesc, (j | k) != 0 ? 1u : 0u);
           umma_commit_pair(empty + s);
         }
-        if constexpr (OP == kAdapt) {
+        if (OP == kAdapt && sg.kind != kProduce) {
           int tm, tn;
-          tile_at(t, m_tiles, n_tiles, tm, tn);
+          tile_at(sg.tile, m_tiles, n_tiles, tm, tn);
           const int* list = p.lists + (size_t)tm * kListStride;
           const int count = list[0], chunks = (p.R + kChunk - 1) / kChunk;
           for (int j = 0; j < count; j++) {
-            if (p.unsafe[list[1 + j]]) continue;
             for (int c = 0; c < chunks; c++, it++) {
               const int s = it % kStages;
               if (!stage_ready(s, it / kStages)) goto done;
@@ -301,101 +349,217 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         umma_commit_pair(acc_full + a);
       }
     }
+  } else if (OP == kAdapt && warp >= 10) {
+    // ------------------------------------------------------------ blocks of low-rank factors
+    const int lt = threadIdx.x - 320, chunks = (p.R + kChunk - 1) / kChunk;
+    uint32_t next = 0;                          // ring stages before this one
+    uint32_t seen = 0;                          // bit s: parity of the next grant of stage s (a stage is granted again only after its block is used up)
+    for (uint32_t tile_i = 0; walk.next(sg); tile_i++) {
+      next += (uint32_t)sg.count;
+      if (sg.kind == kProduce) continue;
+      int tm, tn;
+      tile_at(sg.tile, m_tiles, n_tiles, tm, tn);
+      const int m0 = tm * 256 + (int)crank * 128, n0 = tn * 256 + (int)crank * 128;
+      const int* list = p.lists + (size_t)tm * kListStride;
+      const int count = list[0];
+      // this thread's 16 pieces of 16 bytes of a block: piece lt & 7 of rows lt / 8, + 8, ...
+      int ids[16];
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int row = m0 + (lt >> 3) + 8 * i;
+        ids[i] = row < p.M ? p.ids[row] : -1;
+      }
+      for (int j = 0; j < count; j++) {
+        const int adapter = list[1 + j];
+        const bool all = low_rank_all(low_rank_finite(p, adapter, tn * 256, lt, kLowThreads));
+        for (int c = 0; c < chunks; c++, next++) {
+          uint4 w[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int row = m0 + (lt >> 3) + 8 * i;
+            w[i] = all && ids[i] == adapter ? __ldcg(reinterpret_cast<const uint4*>(p.v + ((size_t)row * chunks + c) * 64) + (lt & 7)) : make_uint4(0, 0, 0, 0);
+          }
+          const int s = next % kStages;
+          if (!low_rank_all(gemm_wait(granted + s, seen >> s & 1u, gw, 1))) goto done;      // all of them or none
+          seen ^= 1u << s;
+          if (!all && lt == 0) unsafe_tile[tile_i % kVerdicts] = tile_i + 1u;      // before the arrival that the MMAs wait for
+          uint8_t *sa = ring + s * kStage, *sb = sa + kOpBytes;
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int r = (lt >> 3) + 8 * i;
+            sts16(sa + r * 128 + (((lt & 7) ^ (r & 7)) << 4), w[i]);
+          }
+          if (!all)
+            for (int i = lt; i < kOpBytes / 16; i += kLowThreads) sts16(sb + 16 * i, make_uint4(0, 0, 0, 0));
+          fence_smem_to_async();
+          low_rank_barrier();
+          if (lt == 0) {
+            const uint32_t lead_full = cluster_addr(full + s, 0u);
+            if (leads) mbar_arrive_expect(full + s, all ? 2 * kOpBytes : 0);
+            else mbar_arrive_cluster(lead_full);
+            if (all) tma_load_2d_pair(sb, &maps.low, c * kChunk, adapter * p.N + n0, lead_full);
+          }
+        }
+      }
+    }
   } else {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3;
-    uint8_t* my_slabs = slabs + q * 2 * kSlab;
-    uint32_t tile_i = 0, stores = 0;
-    // This lane's 32 values, columns 32 `half` .. + 31 of its row of a slab.
-    auto put = [&](uint8_t* slab, int half, const float* v) {
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        sts16(slab + lane * 128 + (((half * 4 + j) ^ (lane & 7)) << 4),
-              make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]), pack_bf16(v[8 * j + 4], v[8 * j + 5]),
-                         pack_bf16(v[8 * j + 6], v[8 * j + 7])));
+    const int q = warp & 3, side = (warp - 2) >> 2;
+    uint8_t* slab = slabs + (warp - 2) * kSlab;
+    uint32_t tile_i = 0;
+    // chunk `j` (16 bytes) of this lane's row of the slab
+    auto put = [&](int j, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+      sts16(slab + lane * 128 + ((j ^ (lane & 7)) << 4), make_uint4(w0, w1, w2, w3));
     };
-    auto next_slab = [&]() {                   // of the two, the one whose store has been read
-      if (lane == 0) bulk_wait_source_free<1>();
+    auto slab_free = [&]() {                   // its last store has been read
+      if (lane == 0) bulk_wait_source_free<0>();
       __syncwarp();
-      return my_slabs + (stores++ & 1u) * kSlab;
     };
-    for (int t = unit; t < tiles; t += units, tile_i++) {
+    auto slab_full = [&]() {
+      fence_smem_to_async();
+      __syncwarp();
+    };
+    // Two groups of 64 accumulator columns per tile: chunks of 32 columns group_chunk(g, 0) and (g, 1).  kGated: 32 gate columns and
+    // the up columns that go with them.
+    auto group_chunk = [&](int g, int which) { return OP == kGated ? 4 * which + 2 * side + g : 4 * side + 2 * g + which; };
+    auto slot = [&](int cta, int c, int i) {   // float4 `i` of 32-column chunk `c`: a warp's rows are 512 contiguous bytes
+      return reinterpret_cast<float4*>(p.partial) + (((size_t)cta * 8 + c) * 8 + i) * 128 + q * 32 + lane;
+    };
+    for (; walk.next(sg); tile_i++) {
       int tm, tn;
-      tile_at(t, m_tiles, n_tiles, tm, tn);
+      tile_at(sg.tile, m_tiles, n_tiles, tm, tn);
       const uint32_t a = tile_i & 1u;
       const int row0 = tm * 256 + (int)crank * 128 + q * 32, n0 = tn * kTileN;
+      const int first_col = n0 + (OP == kGated ? 64 : 128) * side;
+      const bool mine = row0 + lane < p.M;
       const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + a * 256;
+      uint32_t* const flag = p.flags + (size_t)blockIdx.x * kSplitFlags + (warp - 2);      // of this unit's slot
+      float v[2][32], w[2][32];
+      // what the units behind this one have left for a group
+      auto load_shares = [&](int g) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int c = group_chunk(g, h);
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float4 f = __ldcg(slot(blockIdx.x + 2, c, i));
+            w[h][4 * i] = f.x; w[h][4 * i + 1] = f.y; w[h][4 * i + 2] = f.z; w[h][4 * i + 3] = f.w;
+          }
+          for (int j = 2; j <= sg.others; j++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const float4 f = __ldcg(slot(blockIdx.x + 2 * j, c, i));
+              w[h][4 * i] += f.x; w[h][4 * i + 1] += f.y; w[h][4 * i + 2] += f.z; w[h][4 * i + 3] += f.w;
+            }
+          }
+        }
+      };
+      bool good = true;
+      if (sg.kind == kProduce && lane == 0) good = gemm_flag_wait(flag, 0u, gw, 5);
+      if (sg.kind == kFinish)
+        for (int j = 1 + lane; j <= sg.others; j += 32) good = good && gemm_flag_wait(flag + 2 * kSplitFlags * j, 1u, gw, 6);
+      if (!__all_sync(0xffffffffu, good)) break;
+      if (sg.kind == kFinish && mine) load_shares(0);      // in flight while the last K blocks run
       if (!__all_sync(0xffffffffu, gemm_wait(acc_full + a, (tile_i >> 1) & 1u, gw, 4))) break;
       tc_fence_after();
-      if (row0 < p.M) {
-        float v[2][32];
-        if (OP != kGated || p.want_pre) {
-          // all 256 accumulator columns as they are
-          int slow = -1;
-          const float* vrow = nullptr;
-          if constexpr (OP == kAdapt) {
-            const int row = row0 + lane;
-            const int id = row < p.M ? p.ids[row] : -1;
-            if (id >= 0 && id < p.adapters && p.unsafe[id]) { slow = id; vrow = p.v + (size_t)row * p.R; }
+      if (row0 < p.M && first_col < p.N) {
+        int slow = -1;                                     // kAdapt: this row's adapter is added here
+        const __nv_bfloat16* vrow = nullptr;
+        if (OP == kAdapt && sg.kind != kProduce) {
+          const int id = mine ? p.ids[row0 + lane] : -1;
+          if (unsafe_tile[tile_i % kVerdicts] == tile_i + 1u && id >= 0 && id < p.adapters && low_rank_unsafe(p, id, n0)) {
+            slow = id;
+            vrow = p.v + (size_t)(row0 + lane) * ((p.R + kChunk - 1) / kChunk * 64);
           }
-          for (int c = 0; c < 4; c++) {
-            const int col = OP == kGated ? n0 + (c & 1) * 64 : n0 + c * 64;
-            if (col >= p.N) continue;
-            tmem_ld32_issue(tbase + c * 64, v[0]);
-            tmem_ld32_issue(tbase + c * 64 + 32, v[1]);
-            uint8_t* slab = next_slab();
-            tmem_ld_wait();
+        }
+        uint32_t keep[16];                                 // kGated: h of the first group
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          const int col = first_col + (OP == kGated ? 32 : 64) * g;
+          if (OP != kGated && col >= p.N) continue;
+          tmem_ld32_issue(tbase + group_chunk(g, 0) * 32, v[0]);
+          tmem_ld32_issue(tbase + group_chunk(g, 1) * 32, v[1]);
+          tmem_ld_wait();
+          if (sg.kind == kProduce) {
+            if (mine) {
+#pragma unroll
+              for (int i = 0; i < 16; i++) {
+                const float* f = v[i >> 3] + 4 * (i & 7);
+                *slot(blockIdx.x, group_chunk(g, i >> 3), i & 7) = make_float4(f[0], f[1], f[2], f[3]);
+              }
+            }
+            continue;
+          }
+          if (sg.kind == kFinish && mine) {
+#pragma unroll
+            for (int i = 0; i < 64; i++) v[i >> 5][i & 31] += w[i >> 5][i & 31];
+          }
+          if constexpr (OP == kGated) {
+            if (p.want_pre && col < p.N) {
+#pragma unroll
+              for (int which = 0; which < 2; which++) {
+                slab_free();
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                  const float* f = v[which] + 4 * j;
+                  put(j, __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+                }
+                slab_full();
+                if (lane == 0) { tma_store_3d(&maps.pre, col, which, row0, slab); bulk_commit(); }
+              }
+            }
+            if (p.act == FP4AR_ACT_SILU) {
+#pragma unroll
+              for (int i = 0; i < 32; i++) v[0][i] = act_value<FP4AR_ACT_SILU>(v[0][i]) * v[1][i];
+            } else if (p.act == FP4AR_ACT_GELU) {
+#pragma unroll
+              for (int i = 0; i < 32; i++) v[0][i] = act_value<FP4AR_ACT_GELU>(v[0][i]) * v[1][i];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i++) v[0][i] = act_value<FP4AR_ACT_GELU_TANH>(v[0][i]) * v[1][i];
+            }
+            if (g == 0) {
+#pragma unroll
+              for (int i = 0; i < 16; i++) keep[i] = pack_bf16(v[0][2 * i], v[0][2 * i + 1]);
+              if (sg.kind == kFinish && mine) load_shares(1);
+              continue;
+            }
+            slab_free();
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              put(j, keep[4 * j], keep[4 * j + 1], keep[4 * j + 2], keep[4 * j + 3]);
+              const float* f = v[0] + 8 * j;
+              put(4 + j, pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+            }
+            slab_full();
+            if (lane == 0) { tma_store_2d(&maps.out, first_col, row0, slab); bulk_commit(); }
+          } else {
             if constexpr (OP == kAdapt) {
               if (slow >= 0) {
 #pragma unroll
                 for (int i = 0; i < 64; i++)
                   if (col + i < p.N) v[i >> 5][i & 31] += low_rank_dot(vrow, p.b + ((size_t)slow * p.N + col + i) * p.R, p.R);
               }
+              __syncwarp();
             }
-            put(slab, 0, v[0]);
-            put(slab, 1, v[1]);
-            fence_smem_to_async();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (OP == kGated) tma_store_3d(&maps.pre, col, c >> 1, row0, slab);
-              else tma_store_2d(&maps.out, col, row0, slab);
-              bulk_commit();
-            }
-          }
-        }
-        if constexpr (OP == kGated) {
-          for (int c = 0; c < 2; c++) {
-            const int col = n0 + c * 64;
-            if (col >= p.N) continue;
-            uint8_t* slab = next_slab();
-            for (int half = 0; half < 2; half++) {
-              tmem_ld32_issue(tbase + c * 64 + half * 32, v[0]);
-              tmem_ld32_issue(tbase + 128 + c * 64 + half * 32, v[1]);
-              tmem_ld_wait();
-              if (p.act == FP4AR_ACT_SILU) {
+            slab_free();
 #pragma unroll
-                for (int i = 0; i < 32; i++) v[0][i] = act_value<FP4AR_ACT_SILU>(v[0][i]) * v[1][i];
-              } else if (p.act == FP4AR_ACT_GELU) {
-#pragma unroll
-                for (int i = 0; i < 32; i++) v[0][i] = act_value<FP4AR_ACT_GELU>(v[0][i]) * v[1][i];
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; i++) v[0][i] = act_value<FP4AR_ACT_GELU_TANH>(v[0][i]) * v[1][i];
-              }
-              put(slab, half, v[0]);
+            for (int j = 0; j < 8; j++) {
+              const float* f = v[j >> 2] + 8 * (j & 3);
+              put(j, pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
             }
-            fence_smem_to_async();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&maps.out, col, row0, slab);
-              bulk_commit();
-            }
+            slab_full();
+            if (lane == 0) { tma_store_2d(&maps.out, col, row0, slab); bulk_commit(); }
+            if (g == 0 && sg.kind == kFinish && mine) load_shares(1);
           }
         }
       }
       tc_fence_before();
-      mbar_arrive_cluster(cluster_addr(acc_empty + a, 0u));
-      __syncwarp();
+      __syncwarp();                                        // every lane has its accumulators and shares in registers
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty + a, 0u));
+      if (sg.kind == kProduce && lane == 0) { __threadfence(); st_release_gpu(flag, 1u); }
+      if (sg.kind == kFinish)
+        for (int j = 1 + lane; j <= sg.others; j += 32) st_release_gpu(flag + 2 * kSplitFlags * j, 0u);
     }
     if (lane == 0) bulk_wait_done<0>();
   }
@@ -432,17 +596,29 @@ inline bool map_2d(CUtensorMap* m, const void* base, long rows, long cols, int b
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-// [rows][2][cols]: the two projections of every row, each clipped at its own width
+// [rows][2][cols] FP32: the two projections of every row, each clipped at its own width
 inline bool map_pre(CUtensorMap* m, const void* base, long rows, long cols) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)cols, 2, (cuuint64_t)rows}, strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)cols * 4};
-  const cuuint32_t box[3] = {64, 1, 32}, one[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, 2, (cuuint64_t)rows}, strides[2] = {(cuuint64_t)cols * 4, (cuuint64_t)cols * 8};
+  const cuuint32_t box[3] = {32, 1, 32}, one[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+
+// How many units share the tiles that are cut (0: none).  A block takes a unit 0.3 us; writing, reading and adding the partials costs
+// about 10 us, so tiles are cut where that saves the units 48 blocks each on average.  (h of 1031 x 1368, K = 6144: 25 idle blocks of 96,
+// 37.5 us whole, 40.9 cut; 2048 x 2048, K = 8192: 35 of 256, 98.4 and 104.9; 4096 x 2048, K = 6144: 52 of 384, 148.5 and 146.7, K = 8192: 69
+// of 512, 198.1 and 190.5; 256 x 2048, K = 4096: 50 of 64, 29.7 and 29.2, K = 8192: 100 of 128, 49.7 and 33.3.)
+inline int cut_units(int tiles, int kblocks, int units) {
+  const long long waves = (tiles + units - 1) / units, idle = (waves * units - tiles) * kblocks / units;
+  if (idle < 48) return 0;
+  if (tiles >= units) return units;
+  const long long ranges = (long long)tiles * kblocks / 8;
+  return ranges <= tiles ? 0 : ranges < units ? (int)ranges : units;
+}
 
 template <int OP>
 int launch_pair_gemm(const Maps& maps, Params p, cudaStream_t stream) {
@@ -454,7 +630,7 @@ int launch_pair_gemm(const Maps& maps, Params p, cudaStream_t stream) {
   p.timeout_ns = kWaitLimitNs;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kThreads<OP>);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -472,7 +648,16 @@ int launch_pair_gemm(const Maps& maps, Params p, cudaStream_t stream) {
   constexpr int kTileN = OP == kGated ? 128 : 256;
   const long tiles = ((long)p.M + 255) / 256 * (((long)p.N + kTileN - 1) / kTileN);
   if (tiles > 0x7fffffffL) return FP4AR_ERR_ARGUMENT;
-  const int units = tiles < fits ? (int)tiles : fits;
+  const int whole = tiles < fits ? (int)tiles : fits;
+  p.cut_units = cut_units((int)tiles, p.kblocks, fits);
+  int units = p.cut_units > whole ? p.cut_units : whole;
+  std::optional<SplitSpace> space;
+  if (p.cut_units) {
+    space.emplace(stream);
+    p.partial = space->partial();
+    p.flags = space->flags();
+    if (!p.partial) { p.cut_units = 0; units = whole; }
+  }
   cfg.gridDim = dim3(2 * units);
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;

@@ -276,7 +276,7 @@ std::tuple<Tensor, Tensor> op_gated_linear(const Tensor& x, const Tensor& wt, in
   const c10::cuda::CUDAGuard guard(dev);
   if (!out.defined()) out = new_empty({s.M, s.F}, at::kBFloat16, dev);
   Tensor pre;
-  if (want_pre) pre = new_empty({s.M, 2 * s.F}, at::kBFloat16, dev);
+  if (want_pre) pre = new_empty({s.M, 2 * s.F}, at::kFloat, dev);
   ok(api.gated_linear(x.data_ptr(), wt.data_ptr(), (int)s.M, (int)s.F, (int)s.K, (int)act, out.mutable_data_ptr(),
                       want_pre ? pre.mutable_data_ptr() : nullptr, stream_of(dev)), "fp4ar_gated_linear");
   return {std::move(out), std::move(pre)};
@@ -287,7 +287,7 @@ std::tuple<Tensor, Tensor> op_gated_backward(const Tensor& dh, const Tensor& pre
   const GatedShape s(x, wt, act);
   const c10::Device dev = x.device();
   require_matrix(dh, at::kBFloat16, {s.M, s.F}, dev, "dh");
-  require_matrix(pre, at::kBFloat16, {s.M, 2 * s.F}, dev, "pre");
+  require_matrix(pre, at::kFloat, {s.M, 2 * s.F}, dev, "pre");
   const c10::cuda::CUDAGuard guard(dev);
   Tensor dx, dw;
   if (!need_dx && !need_dw) return {dx, dw};

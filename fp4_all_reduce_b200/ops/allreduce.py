@@ -186,7 +186,7 @@ def _(x, wt, activation):
 
 @torch.library.register_fake("fp4ar::gated_linear_pre")
 def _(x, wt, activation):
-    return x.new_empty((x.shape[0], wt.shape[0] // 2)), x.new_empty((x.shape[0], wt.shape[0]))
+    return x.new_empty((x.shape[0], wt.shape[0] // 2)), x.new_empty((x.shape[0], wt.shape[0]), dtype=torch.float32)
 
 
 @torch.library.register_fake("fp4ar::gated_linear_backward")

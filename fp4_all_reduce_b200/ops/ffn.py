@@ -10,8 +10,8 @@ returns, h is the input of the row-parallel linear behind it.  Under tensor para
 gradient, to be summed by `ctx.all_reduce`.
 
 BF16 tensors, contiguous, starting on 16-byte boundaries; K and F are multiples of 8, M is any row count.  Sums, the activation and
-the product are FP32, h is rounded once.  The backward pass takes the projections, and hands their gradients to its matrix
-products, in BF16.  Everything runs on the current stream.
+the product are FP32, h is rounded once.  The backward pass hands the gradients of
+the projections to its matrix products in BF16.  Everything runs on the current stream.
 """
 from __future__ import annotations
 
@@ -53,7 +53,7 @@ def gated_linear(x: torch.Tensor, wt: torch.Tensor, activation: int = N.ACT_SILU
 
 def gated_linear_forward(x: torch.Tensor, wt: torch.Tensor, activation: int = N.ACT_SILU, *,
                          out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """(h, pre): pre [M, 2 F] holds the gate and the up projections in BF16; h is the same as without it.  Records no gradient."""
+    """(h, pre): pre [M, 2 F] holds the gate and the up projections in FP32; h is the same as without it.  Records no gradient."""
     return N.front().gated_linear(x, wt, activation, True, out)
 
 

@@ -39,12 +39,11 @@ def gated(x, wt, kind):
 
 
 def gated_grads(dh, x, wt, kind):
-    """(dx, dwt, their bounds).  |a'| <= 1.13 and |a''| <= 0.8; the projections and dpre are rounded to BF16, the results too."""
+    """(dx, dwt, their bounds).  |a'| <= 1.13 and |a''| <= 0.8; dpre is rounded to BF16, the results too."""
     _, g, u, _, eg, eu = gated(x, wt, kind)
     x, wt, dh = x.detach().double(), wt.detach().double(), dh.double()
     dg, du = dh * u * act_grad(g, kind), dh * act(g, kind)
     dpre = torch.cat([dg, du], 1)
-    eg, eu = eg + BF16 * g.abs(), eu + BF16 * u.abs()
     small = 2.0 ** -18
     edg = dh.abs() * (0.8 * eg * (u.abs() + eu) + 1.13 * eu) + (BF16 + small) * dg.abs() + small * dh.abs() * u.abs()
     edu = dh.abs() * 1.13 * eg + (BF16 + small) * du.abs()

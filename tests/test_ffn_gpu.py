@@ -19,8 +19,8 @@ def _data(M, K, F, seed=0):
     return x, wt, dh
 
 
-def _within(got, want, bound):
-    assert got.shape == want.shape and got.dtype == torch.bfloat16
+def _within(got, want, bound, dtype=torch.bfloat16):
+    assert got.shape == want.shape and got.dtype == dtype
     d = (got.double() - want).abs()
     assert bool((d <= bound).all()), float((d / bound).max())
 
@@ -39,7 +39,7 @@ def test_forward(M, K, F, act):
     _within(h, want, bound)
     h2, pre = ffn.gated_linear_forward(x, wt, act)
     assert torch.equal(h, h2)
-    _within(pre, torch.cat([gate, up], 1), torch.cat([eg + R.BF16 * gate.abs(), eu + R.BF16 * up.abs()], 1) + 1e-30)
+    _within(pre, torch.cat([gate, up], 1), torch.cat([eg, eu], 1) + 1e-30, torch.float32)
     assert G.gemm_status().code == 0
 
 
@@ -53,8 +53,7 @@ def test_gradients(M, K, F, act):
     wx, ww, bx, bw = R.gated_grads(dh, x, wt, act)
     _within(dx, wx, bx)
     _within(dw, ww, bw)
-    # Four roundings (gate, up, dpre, result) of at most 2^-8 each are independent: their rms is below 2^-8 sqrt(4 / 3), and
-    # a'' g may take the gate's above its share
+    # two roundings (dpre, result) of at most 2^-8 each, of independent sizes: their rms is below 2^-8 sqrt(2 / 3)
     for got, want in ((dx, wx), (dw, ww)):
-        assert (got.double() - want).norm() <= 2 ** -7 * want.norm()
+        assert (got.double() - want).norm() <= R.BF16 * want.norm()
     assert G.gemm_status().code == 0
