@@ -2,7 +2,6 @@
 //
 // Two launches: a first kernel computes V[i] = s_a x_i A_a^T and lists the adapters of every 256 rows; the product with W then takes
 // V_a B_a^T into the same accumulators (layer_gemm.cuh).
-#include <cooperative_groups.h>
 #include "layer_gemm.cuh"
 
 namespace fp4ar {
@@ -23,185 +22,239 @@ struct Workspace {
 };
 
 struct LowParams {
-  const __nv_bfloat16 *x, *a;
+  int M, R, adapters, kblocks, split;
   const int* ids;
   const float* scales;
-  int M, K, R, adapters, split;
   __nv_bfloat16* v;
   int* lists;
+  StatusWords* status;
+  unsigned long long timeout_ns;
 };
 
-__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
+// V of 128 rows, the first launch.  x goes once through shared memory for all adapters of the rows: B of the product are the A_a of up to
+// 256 / R of them, one behind the other (more adapters take more passes), every row is multiplied with all of them, and the
+// epilogue keeps of each row the columns of its own adapter.  So what another adapter or row holds reaches nobody else, and the
+// time is that of reading x.  A cluster of `split` CTAs cuts K where there are few rows; their sums meet in shared memory, in the
+// order of the CTAs.
+constexpr int kLowStages = 4;
+constexpr int kLowStage = kOpBytes + 256 * kBlockK * 2;        // x, then up to 256 rows of A
+__host__ __device__ constexpr int low_stages(int R) { return R <= 64 ? 4 : 3; }
+__host__ __device__ constexpr int low_smem(int R) { return low_stages(R) * kLowStage + 128 * R * 4 + 1024; }
 
-// The distinct adapters of 256 rows in the order of their first rows, by 256 threads.
-__device__ void list_adapters(const LowParams& p, int tile, int* sid, int* scount) {
-  const int tid = threadIdx.x, row = tile * 256 + tid;
-  int id = row < p.M ? p.ids[row] : -1;
-  if (id >= p.adapters) id = -1;
-  sid[tid] = id;
-  __syncthreads();
-  bool first = id >= 0;
-  for (int s = 0; s < tid; s++) first = first && sid[s] != id;
-  const uint32_t votes = __ballot_sync(0xffffffffu, first);
-  if ((tid & 31) == 0) scount[tid >> 5] = __popc(votes);
-  __syncthreads();
-  int before = __popc(votes & ((1u << (tid & 31)) - 1u)), total = 0;
-  for (int w = 0; w < 8; w++) {
-    if (w < tid >> 5) before += scount[w];
-    total += scount[w];
+__global__ void __launch_bounds__(192, 1)
+low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ LowParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kLowStages], empty[kLowStages], acc_full, acc_empty;
+  __shared__ uint32_t tmem_holder;
+  __shared__ volatile uint32_t abort_flag;
+  __shared__ int sid[256], list[128], scount[8], count;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int stages = low_stages(p.R);
+  float* part = reinterpret_cast<float*>(ring + stages * kLowStage);       // [128][R]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tile = blockIdx.x / p.split, crank = blockIdx.x % p.split, row0 = tile * 128;
+  if (tid == 0) {
+    for (int s = 0; s < stages; s++) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
+    mbar_init(&acc_full, 1);
+    mbar_init(&acc_empty, 4);
+    abort_flag = 0u;
+    mbar_init_fence();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_a);
   }
-  int* list = p.lists + (size_t)tile * kListStride;
-  if (first) list[1 + before] = id;
-  if (tid == 0) list[0] = total;
-}
-
-// V of 64 rows x 8 NT ranks: a cluster of `split` CTAs cuts K, the eight warps of a CTA cut its share, and the sums meet in shared
-// memory, warps first, CTAs next, always in the same order.
-//
-// A warp takes 32 K columns at a time.  Operands go from global memory to registers without a stop: a lane's 16 bytes of a row are
-// columns 8 t .. 8 t + 7 of the 32 (t = lane & 3), and since x and A use the same columns, their order inside the product does
-// not matter: words 0, 1 are one mma.sync m16n8k16, words 2, 3 the next.  (tcgen05 has nothing to give here: the product has a
-// third of the operations per byte that would make it matter, and a tile of x would have to go through shared memory for every
-// adapter in it.)  x of the next 32 columns is in flight during the products.
-// Rows of a tile with several adapters: one pass for each, over the groups of 16 rows that have it, and of its results only those
-// rows are kept, so what another adapter holds reaches nobody else.
-// Bound by the reads of x: ...
-template <int NT>
-__global__ void __launch_bounds__(256, 1) low_rank_kernel(const __grid_constant__ LowParams p) {
-  constexpr int kCols = 8 * NT;
-  extern __shared__ float red[];                        // [8 warps][64 rows][kCols], then the CTA's sums [64][kCols]
-  __shared__ int sid[256];
-  __shared__ int scount[8];
-  float* part = red + 8 * 64 * kCols;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, t = lane & 3;
-  const int tile = blockIdx.x / p.split, crank = blockIdx.x % p.split, row0 = tile * 64;
+  if (warp == 1) { tmem_alloc(&tmem_holder, 256); tmem_relinquish(); }
+  GemmWait gw{&abort_flag, p.status, p.timeout_ns};
   pdl_wait_prior_grids();
   pdl_release_dependents();
-  if ((tile & 3) == 0 && crank == 0) list_adapters(p, tile >> 2, sid, scount);
 
-  // both halves of the tile's ids
-  int id0 = row0 + lane < p.M ? p.ids[row0 + lane] : -1, id1 = row0 + 32 + lane < p.M ? p.ids[row0 + 32 + lane] : -1;
-  if (id0 < 0 || id0 >= p.adapters) id0 = -1;
-  if (id1 < 0 || id1 >= p.adapters) id1 = -1;
-  const unsigned long long have = ((unsigned long long)__ballot_sync(0xffffffffu, id1 >= 0) << 32) | __ballot_sync(0xffffffffu, id0 >= 0);
-  const int chunks = (p.K + 31) / 32, step = 8 * p.split;
+  // the distinct adapters of the 128 rows, in the order of their first rows; thread 64 + r has row r
+  auto id_of = [&](int row) {
+    const int id = row < p.M ? p.ids[row] : -1;
+    return id < p.adapters ? id : -1;
+  };
+  const int r = tid - 64;
+  int id = -1;
+  bool first = false;
+  uint32_t votes = 0;
+  if (r >= 0) sid[r] = id = id_of(row0 + r);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (r >= 0) {
+    first = id >= 0;
+    for (int i = 0; i < r; i++) first = first && sid[i] != id;
+    votes = __ballot_sync(0xffffffffu, first);
+    if (lane == 0) scount[warp - 2] = __popc(votes);
+  }
+  __syncthreads();
+  if (first) {
+    int at = __popc(votes & ((1u << lane) - 1u));
+    for (int w = 0; w < warp - 2; w++) at += scount[w];
+    list[at] = id;
+  }
+  if (tid == 64) count = scount[0] + scount[1] + scount[2] + scount[3];
+  __syncthreads();
+  const uint32_t tmem_base = tmem_holder;
+  const int rp = (p.R + 15) / 16 * 16, group = 256 / rp, passes = (count + group - 1) / group;
+  const int kb0 = p.kblocks * crank / p.split, kb1 = p.kblocks * (crank + 1) / p.split;
+  int issued = 0;
 
-  for (int r0 = 0; r0 < p.R; r0 += kCols) {
-    for (unsigned long long left = have; left;) {
-      const int f = __ffsll((long long)left) - 1;
-      const int adapter = __shfl_sync(0xffffffffu, f < 32 ? id0 : id1, f & 31);
-      const unsigned long long rows = ((unsigned long long)__ballot_sync(0xffffffffu, id1 == adapter) << 32) | __ballot_sync(0xffffffffu, id0 == adapter);
-      left &= ~rows;
-      float acc[4][NT][4];
-#pragma unroll
-      for (int m = 0; m < 4; m++)
-#pragma unroll
-        for (int n = 0; n < NT; n++) acc[m][n][0] = acc[m][n][1] = acc[m][n][2] = acc[m][n][3] = 0.0f;
-      const __nv_bfloat16* a = p.a + (size_t)adapter * p.R * p.K;
-      auto x_word = [&](int m, int half, int k) {        // 8 columns of row 16 m + 8 half + grp
-        const int row = row0 + 16 * m + 8 * half + grp;
-        return (rows >> (16 * m) & 0xFFFFull) && row < p.M && k < p.K ? ldg16(p.x + (size_t)row * p.K + k) : make_uint4(0, 0, 0, 0);
-      };
-      int c = crank * 8 + warp;
-      uint4 xs[4][2];
-      if (c < chunks) {
-#pragma unroll
-        for (int m = 0; m < 4; m++) { xs[m][0] = x_word(m, 0, c * 32 + 8 * t); xs[m][1] = x_word(m, 1, c * 32 + 8 * t); }
-      }
-      for (; c < chunks; c += step) {
-        const int k = c * 32 + 8 * t, next = k + 32 * step;
-        uint4 as[NT];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const int r = r0 + 8 * n + grp;
-          as[n] = r < p.R && k < p.K ? __ldg(reinterpret_cast<const uint4*>(a + (size_t)r * p.K + k)) : make_uint4(0, 0, 0, 0);
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int ps = 0; ps < passes; ps++) {
+        const int n = min(group, count - ps * group);
+        for (int kb = kb0; kb < kb1; kb++, issued++) {
+          const int s = issued % stages;
+          if (!gemm_wait(empty + s, ((issued / stages) & 1u) ^ 1u, gw, 1)) goto done;
+          uint8_t* at = ring + s * kLowStage;
+          mbar_arrive_expect(full + s, kOpBytes + n * rp * 128);
+          tma_load_2d(at, &map_x, kb * kBlockK, row0, full + s);
+          for (int i = 0; i < n; i++) tma_load_2d(at + kOpBytes + i * rp * 128, &map_a, kb * kBlockK, list[ps * group + i] * p.R, full + s);
         }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int it = 0;
+      for (int ps = 0; ps < passes; ps++) {
+        const int n = min(group, count - ps * group) * rp;
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+        if (!gemm_wait(&acc_empty, (ps & 1u) ^ 1u, gw, 2)) goto done;
+        tc_fence_after();
+        for (int kb = kb0; kb < kb1; kb++, it++) {
+          const int s = it % stages;
+          if (!gemm_wait(full + s, (it / stages) & 1u, gw, 3)) goto done;
+          tc_fence_after();
+          const uint64_t da = umma_desc_k128(ring + s * kLowStage), db = umma_desc_k128(ring + s * kLowStage + kOpBytes);
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
-          const uint4 x0 = xs[m][0], x1 = xs[m][1];
-          xs[m][0] = x_word(m, 0, next);
-          xs[m][1] = x_word(m, 1, next);
-          if (rows >> (16 * m) & 0xFFFFull) {
+          for (int k = 0; k < kBlockK / 16; k++) umma_bf16(tmem_base, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, kb > kb0 || k ? 1u : 0u);
+          umma_commit(empty + s);
+        }
+        umma_commit(&acc_full);
+      }
+    }
+  } else {
+    // warps 2-5: TMEM lane quarter warp & 3 has rows 32 (warp & 3) ...
+    const int q = warp & 3, row = q * 32 + lane;
+    const int mine = sid[row];
+    for (int ps = 0; ps < passes; ps++) {
+      if (!__all_sync(0xffffffffu, gemm_wait(&acc_full, ps & 1u, gw, 4))) break;
+      tc_fence_after();
+      const int n = min(group, count - ps * group);
+      for (int i = 0; i < n; i++) {
+        const bool take = mine == list[ps * group + i];
+        if (!__any_sync(0xffffffffu, take)) continue;
+        for (int c = 0; c < rp; c += 32) {               // beyond rp: columns of the next adapter or unused ones (256 + 16 are never reached: rp = 16 then)
+          float v[32];
+          const uint32_t at = tmem_base + ((uint32_t)(q * 32) << 16) + i * rp + c;
+          const int cols = min(32, rp - c);
+          if (cols == 32) tmem_ld32_issue(at, v); else tmem_ld16_issue(at, v);
+          tmem_ld_wait();
+          if (take) {
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-              mma_bf16(acc[m][n], x0.x, x1.x, x0.y, x1.y, as[n].x, as[n].y);
-              mma_bf16(acc[m][n], x0.z, x1.z, x0.w, x1.w, as[n].z, as[n].w);
-            }
+            for (int e = 0; e < 32; e += 4)
+              if (c + e < p.R) *reinterpret_cast<float4*>(part + row * p.R + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
           }
         }
       }
-      // rows 16 m + grp and + 8 of this adapter, columns 8 n + 2 t, + 1
-#pragma unroll
-      for (int m = 0; m < 4; m++)
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-          const int r = 16 * m + 8 * half + grp;
-          if (rows >> r & 1ull) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-              *reinterpret_cast<float2*>(red + (warp * 64 + r) * kCols + 8 * n + 2 * t) = make_float2(acc[m][n][2 * half], acc[m][n][2 * half + 1]);
-          }
-        }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty);
+    }
+  }
+done:
+  tc_fence_before();
+  __syncthreads();
+  if (abort_flag != 0u) {
+    if (tid == 0)
+      for (int i = max(0, issued - stages); i < issued; i++) gemm_settle(full + i % stages, (i / stages) & 1);
+    if (tid == 32) {
+      __shared__ uint64_t settled;
+      mbar_init(&settled, 1);
+      umma_commit(&settled);
+      gemm_settle(&settled, 0u);
     }
     __syncthreads();
-    for (int i = tid; i < 64 * kCols; i += 256) {
-      float s = 0.0f;
-      if (have >> (i / kCols) & 1ull) {
-#pragma unroll
-        for (int w = 0; w < 8; w++) s += red[w * 64 * kCols + i];
-      }
-      part[i] = s;
-    }
-    if (p.split > 1) cooperative_groups::this_cluster().sync(); else __syncthreads();
-    const int share = 64 / p.split, padded = (p.R + kChunk - 1) / kChunk * kChunk;
-    for (int i = tid; i < share * kCols; i += 256) {
-      const int r = crank * share + i / kCols, n = i % kCols;
-      if (!(have >> r & 1ull) || r0 + n >= padded) continue;
-      float s = 0.0f;
+  }
+  if (p.split > 1) cluster_sync_all();
+  // this CTA's share of the rows: the sum of the cluster's parts, scaled, as two BF16 halves
+  const int share = 128 / p.split, padded = (p.R + kChunk - 1) / kChunk * kChunk;
+  for (int i = tid; i < share * (padded / 2); i += 192) {
+    const int rr = crank * share + i / (padded / 2), n = i % (padded / 2) * 2;
+    const int a = sid[rr];
+    if (a < 0) continue;                                 // nobody reads its V
+    float2 s = make_float2(0.0f, 0.0f);
+    if (n < p.R) {
       for (int d = 0; d < p.split; d++) {
-        const float* from = p.split > 1 ? cooperative_groups::this_cluster().map_shared_rank(part, d) : part;
-        s += from[r * kCols + n];
+        float2 f;
+        if (p.split > 1)
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(cluster_addr(part + rr * p.R + n, d)));
+        else
+          f = *reinterpret_cast<const float2*>(part + rr * p.R + n);
+        s.x += f.x;
+        s.y += f.y;
       }
-      if (p.scales) s *= p.scales[p.ids[row0 + r]];
-      // the rounded value and what the rounding left; what is not finite stays in the first alone
-      const __nv_bfloat16 hi = __float2bfloat16_rn(s);
-      const float left = s - __bfloat162float(hi);
-      __nv_bfloat16* line = p.v + (size_t)(row0 + r) * (2 * padded) + (r0 + n) / kChunk * 64 + n % kChunk;
-      line[0] = hi;
-      line[kChunk] = __float2bfloat16_rn(fabsf(left) <= 3.4e38f ? left : 0.0f);
+      if (p.scales) { const float sc = p.scales[a]; s.x *= sc; s.y *= sc; }
     }
-    if (p.split > 1) cooperative_groups::this_cluster().sync(); else __syncthreads();
+    // the rounded value and what the rounding left; what is not finite stays in the first alone
+    const uint32_t hi = pack_bf16(s.x, s.y);
+    const float l0 = s.x - bf16_lo(hi), l1 = s.y - bf16_hi(hi);
+    uint32_t* line = reinterpret_cast<uint32_t*>(p.v + (size_t)(row0 + rr) * (2 * padded) + n / kChunk * 64 + n % kChunk);
+    line[0] = hi;
+    line[kChunk / 2] = pack_bf16(fabsf(l0) <= 3.4e38f ? l0 : 0.0f, fabsf(l1) <= 3.4e38f ? l1 : 0.0f);
+  }
+  if ((tile & 1) == 0 && crank == 0) {
+    // the list of 256 rows for the product with W: these 128 rows' and what the other 128 add
+    __syncthreads();
+    if (r >= 0) sid[128 + r] = id = id_of(row0 + 128 + r);
+    __syncthreads();
+    if (r >= 0) {
+      first = id >= 0;
+      for (int i = 0; i < 128 + r; i++) first = first && sid[i] != id;
+      votes = __ballot_sync(0xffffffffu, first);
+      if (lane == 0) scount[warp - 2] = __popc(votes);
+    }
+    __syncthreads();
+    int* out = p.lists + (size_t)(tile >> 1) * kListStride;
+    for (int i = tid; i < count; i += 192) out[1 + i] = list[i];
+    if (first) {
+      int at = count + __popc(votes & ((1u << lane) - 1u));
+      for (int w = 0; w < warp - 2; w++) at += scount[w];
+      out[1 + at] = id;
+    }
+    if (tid == 64) out[0] = count + scount[0] + scount[1] + scount[2] + scount[3];
+  }
+  if (p.split > 1) cluster_sync_all();                   // a CTA's part is read until here
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 256);
   }
 }
 
-template <int NT>
-static int launch_low_rank(LowParams p, cudaStream_t stream) {
-  constexpr int kBytes = 9 * 64 * 8 * NT * 4;
+static int launch_low_rank(const void* x, const void* a, int K, LowParams p, cudaStream_t stream) {
   static std::atomic<int> raised[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cuda_fail();
   if (!raised[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(low_rank_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess) return cuda_fail();
+    if (cudaFuncSetAttribute(low_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, low_smem(64) > low_smem(128) ? low_smem(64) : low_smem(128)) != cudaSuccess)
+      return cuda_fail();
     raised[dev].store(1, std::memory_order_release);
   }
-  // as many CTAs per 64 rows, up to eight, as the SMs have room for
-  const int tiles = (p.M + 63) / 64, sms = device_sm_count(), chunks = (p.K + 31) / 32;
+  p.status = gemm_status_word();
+  if (!p.status) return cuda_fail();
+  p.timeout_ns = kWaitLimitNs;
+  CUtensorMap mx, ma;
+  if (!map_2d(&mx, x, p.M, K, 128) || !map_2d(&ma, a, (long)p.adapters * p.R, K, (p.R + 15) / 16 * 16)) return FP4AR_ERR_UNSUPPORTED;
+  // as many CTAs per 128 rows, up to eight, as the SMs have room for
+  const int tiles = (p.M + 127) / 128, sms = device_sm_count();
   p.split = 1;
-  while (p.split < 8 && 2 * p.split * tiles <= sms && 16 * p.split <= chunks) p.split *= 2;
+  while (p.split < 8 && 2 * p.split * tiles <= sms && 2 * p.split <= p.kblocks) p.split *= 2;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(tiles * p.split);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = kBytes;
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = low_smem(p.R);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -210,7 +263,7 @@ static int launch_low_rank(LowParams p, cudaStream_t stream) {
   attr[1].val.clusterDim.x = p.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.split > 1 ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, low_rank_kernel<NT>, p) != cudaSuccess) return cuda_fail();
+  if (cudaLaunchKernelEx(&cfg, low_rank_kernel, mx, ma, p) != cudaSuccess) return cuda_fail();
   return cuda_check_launch();
 }
 
@@ -240,8 +293,11 @@ extern "C" int fp4ar_linear_adapters(const void* x, const void* wt, const int* i
     return FP4AR_ERR_ARGUMENT;
   const cudaStream_t stream = (cudaStream_t)stream_;
   const Workspace ws(workspace, M, R);
-  const LowParams lp{(const __nv_bfloat16*)x, (const __nv_bfloat16*)a, ids, scales, M, K, R, adapters, 1, ws.v, ws.lists};
-  const int rc = R <= 16 ? launch_low_rank<2>(lp, stream) : R <= 32 ? launch_low_rank<4>(lp, stream) : launch_low_rank<8>(lp, stream);
+  LowParams lp;
+  memset(&lp, 0, sizeof(lp));
+  lp.M = M; lp.R = R; lp.adapters = adapters; lp.kblocks = (K + 63) / 64;
+  lp.ids = ids; lp.scales = scales; lp.v = ws.v; lp.lists = ws.lists;
+  const int rc = launch_low_rank(x, a, K, lp, stream);
   if (rc != FP4AR_OK) return rc;
   Maps maps;
   memset(&maps, 0, sizeof(maps));

@@ -185,17 +185,21 @@ __device__ __forceinline__ bool low_rank_all(bool yes) {
   return v != 0;
 }
 
+// Not zero where one of two BF16 values is infinite or NaN (all eight exponent bits set).
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
 // Rows n0 .. n0 + 255 (below N) of B of one adapter: are all values finite?  By `lanes` lanes, each with its own answer.
 __device__ __forceinline__ bool low_rank_finite(const Params& p, int adapter, int n0, int lane, int lanes) {
   const uint4* b = reinterpret_cast<const uint4*>(p.b + ((size_t)adapter * p.N + n0) * p.R);
   const int n = min(256, p.N - n0) * (p.R / 8);
-  bool bad = false;
-#pragma unroll 8
-  for (int i = lane; i < n; i += lanes) {
-    const uint4 w = b[i];
-    for (uint32_t e : {w.x, w.y, w.z, w.w}) bad = bad || (e & 0x7F80u) == 0x7F80u || (e & 0x7F800000u) == 0x7F800000u;
+  uint32_t bad = 0;
+  for (int i = lane; i < n; i += 16 * lanes) {               // sixteen loads in flight
+    uint4 w[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) w[j] = i + j * lanes < n ? __ldg(b + i + j * lanes) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 16; j++) bad |= not_finite(w[j].x) | not_finite(w[j].y) | not_finite(w[j].z) | not_finite(w[j].w);
   }
-  return !bad;
+  return bad == 0;
 }
 static __device__ __noinline__ bool low_rank_unsafe(const Params& p, int adapter, int n0) { return !low_rank_finite(p, adapter, n0, 0, 1); }
 
@@ -237,7 +241,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   Seg sg;
 
   if (threadIdx.x == 0) {
-    // kAdapt: both producers announce a stage, since both may write into it themselves
+    // kAdapt: two arrivals, since both CTAs write into a stage of low-rank factors themselves
     for (int s = 0; s < kStages; s++) { mbar_init(full + s, OP == kAdapt ? 2 : 1); mbar_init(empty + s, 1); mbar_init(granted + s, 1); }
     for (int a = 0; a < 2; a++) { mbar_init(acc_full + a, 1); mbar_init(acc_empty + a, 16); }
     mbar_init(settled, 1);
@@ -272,8 +276,12 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
           if (!gemm_wait(empty + s, ((issued / kStages) & 1u) ^ 1u, gw, 1)) goto done;
           uint8_t *sa = ring + s * kStage, *sb = sa + kOpBytes;
           const uint32_t lead_full = cluster_addr(full + s, 0u);
-          if (leads) mbar_arrive_expect(full + s, 2 * kStage);
-          else if (OP == kAdapt) mbar_arrive_cluster(lead_full);
+          if (leads) {
+            mbar_arrive_expect(full + s, 2 * kStage);
+            // (the second arrival is the other CTA's for a block of low-rank factors alone: one at cluster scope for every K
+            // block, and a wait at that scope, cost 90 us of 165 at M = 4096, K = 2048)
+            if (OP == kAdapt) mbar_arrive(full + s);
+          }
           const int k0 = kb * kBlockK;
           if constexpr (kAMn) {
             tma_load_2d_pair(sa, &maps.a, m0, k0, lead_full);
@@ -304,11 +312,6 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && leads) {
       uint32_t it = 0, tile_i = 0;
-      auto stage_ready = [&](int s, uint32_t round) {
-        if constexpr (OP != kAdapt) return gemm_wait(full + s, round & 1u, gw, 3);
-        // the second wait takes what the other CTA's producer wrote, at cluster scope
-        else return gemm_wait(full + s, round & 1u, gw, 3) && mbar_test_cluster(full + s, round & 1u);
-      };
       for (; walk.next(sg); tile_i++) {
         const uint32_t a = tile_i & 1u;
         if (!gemm_wait(acc_empty + a, ((tile_i >> 1) & 1u) ^ 1u, gw, 2)) goto done;
@@ -316,7 +319,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         const uint32_t d = tmem_base + a * 256;
         for (int j = 0; j < sg.count; j++, it++) {
           const int s = it % kStages;
-          if (!stage_ready(s, it / kStages)) goto done;
+          if (!gemm_wait(full + s, (it / kStages) & 1u, gw, 3)) goto done;
           tc_fence_after();
           const uint8_t* sa = ring + s * kStage;
           const uint64_t da = kAMn ? umma_desc_mn128(sa) : umma_desc_k128(sa);
@@ -334,7 +337,8 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
           for (int j = 0; j < count; j++) {
             for (int c = 0; c < chunks; c++, it++) {
               const int s = it % kStages;
-              if (!stage_ready(s, it / kStages)) goto done;
+              if (!gemm_wait(full + s, (it / kStages) & 1u, gw, 3)) goto done;
+              mbar_test_cluster(full + s, (it / kStages) & 1u);      // through by now: takes what the other CTA's warps wrote
               tc_fence_after();
               const uint64_t da = umma_desc_k128(ring + s * kStage), db = umma_desc_k128(ring + s * kStage + kOpBytes);
               const int steps = (min(kChunk, p.R - c * kChunk) + 15) / 16;
