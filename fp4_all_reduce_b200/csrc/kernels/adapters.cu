@@ -2,6 +2,7 @@
 //
 // Two launches: a first kernel computes V[i] = s_a x_i A_a^T and lists the adapters of every 256 rows; the product with W then takes
 // V_a B_a^T into the same accumulators (layer_gemm.cuh).
+#include "few_rows.cuh"
 #include "layer_gemm.cuh"
 
 namespace fp4ar {
@@ -267,6 +268,52 @@ static int launch_low_rank(const void* x, const void* a, int K, LowParams p, cud
   return cuda_check_launch();
 }
 
+__device__ __forceinline__ uint4 ldg16(const uint4* p) {      // volatile: issued in the order written, ahead of the arithmetic
+  uint4 r;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
+// V of few rows: eight ranks of a row per CTA, a warp for each.  Bound by latency: a row of A_a is K numbers, eight loads of every lane in
+// flight.
+__global__ void __launch_bounds__(256) few_low_rank_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ a,
+                                                           const int* __restrict__ ids, const float* __restrict__ scales, int K, int R, int adapters,
+                                                           __nv_bfloat16* __restrict__ v) {
+  pdl_wait_prior_grids();
+  pdl_release_dependents();                              // after the wait: the product with W relies on it
+  const int row = blockIdx.x, r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int id = ids[row];
+  if (id < 0 || id >= adapters) return;                  // nobody reads its V
+  const uint4* xp = reinterpret_cast<const uint4*>(x + (size_t)row * K);
+  const uint4* ap = reinterpret_cast<const uint4*>(a + ((size_t)id * R + r) * K);
+  float s = 0.0f;
+  for (int i = lane; i < K / 8; i += 256) {
+    uint4 xv[8], av[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const bool in = i + 32 * j < K / 8;
+      av[j] = in ? ldg16(ap + i + 32 * j) : make_uint4(0, 0, 0, 0);
+      xv[j] = in ? ldg16(xp + i + 32 * j) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const uint32_t xw[4] = {xv[j].x, xv[j].y, xv[j].z, xv[j].w}, aw[4] = {av[j].x, av[j].y, av[j].z, av[j].w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) s = fmaf(bf16_hi(xw[e]), bf16_hi(aw[e]), fmaf(bf16_lo(xw[e]), bf16_lo(aw[e]), s));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) {
+    if (scales) s *= scales[id];
+    const __nv_bfloat16 hi = __float2bfloat16_rn(s);
+    const float left = s - __bfloat162float(hi);
+    __nv_bfloat16* line = v + ((size_t)row * ((R + kChunk - 1) / kChunk) + r / kChunk) * 64 + r % kChunk;
+    line[0] = hi;
+    line[kChunk] = __float2bfloat16_rn(fabsf(left) <= 3.4e38f ? left : 0.0f);
+  }
+}
+
 }  // namespace layer
 }  // namespace fp4ar
 
@@ -293,6 +340,25 @@ extern "C" int fp4ar_linear_adapters(const void* x, const void* wt, const int* i
     return FP4AR_ERR_ARGUMENT;
   const cudaStream_t stream = (cudaStream_t)stream_;
   const Workspace ws(workspace, M, R);
+  if (M <= kFewRows) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(M, R / 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, few_low_rank_kernel, (const __nv_bfloat16*)x, (const __nv_bfloat16*)a, ids, scales, K, R, adapters, ws.v) != cudaSuccess)
+      return cuda_fail();
+    FewParams fp;
+    memset(&fp, 0, sizeof(fp));
+    fp.M = M; fp.N = N; fp.out = (__nv_bfloat16*)y;
+    fp.R = R; fp.adapters = adapters; fp.ids = ids; fp.v = ws.v; fp.b = (const __nv_bfloat16*)b;
+    return launch_few_rows<kAdapt>(wt, N, x, K, fp, stream);
+  }
   LowParams lp;
   memset(&lp, 0, sizeof(lp));
   lp.M = M; lp.R = R; lp.adapters = adapters; lp.kblocks = (K + 63) / 64;

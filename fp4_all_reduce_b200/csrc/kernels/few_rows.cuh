@@ -1,0 +1,248 @@
+// The same products for few rows (M <= 128), where the time is that of reading the weights once.
+//
+// The operands change sides: 128 rows of W are the M of the tcgen05 product and the rows of x its N (16 .. 128), so nothing is
+// multiplied for rows that are not there.  A CTA of its own for every 128 rows of W would leave SMs idle and the others with
+// a long chain of K blocks, so a cluster of up to eight CTAs cuts K: each leaves its FP32 sums in shared memory, and all of them add
+// up a share of the outputs, in the order of the CTAs.  Two CTAs fit an SM, one's set-up and sums run under the other's loads.
+//   kGated   the 128 rows are 64 gate rows and the 64 up rows that go with them: their product is taken where the sums meet
+//   kAdapt   the low-rank part of an output is added there too, by plain FP32 products with V.  V comes from a launch before this
+//            one; only that step waits for it (see below), the weights are on their way meanwhile
+#pragma once
+#include "layer_gemm.cuh"
+
+namespace fp4ar {
+namespace layer {
+
+constexpr int kFewRows = 128, kFewStagesMax = 8;
+
+struct FewParams {
+  int M, N, kblocks, split, stages, tokens;      // tokens: M rounded up to 16; N: columns of the output
+  int act;
+  __nv_bfloat16* out;
+  float* pre;                                    // kGated, optional [M][2 N]
+  // kAdapt, as in Params
+  int R, adapters;
+  const int* ids;
+  const __nv_bfloat16* v;
+  const __nv_bfloat16* b;
+  StatusWords* status;
+  unsigned long long timeout_ns;
+};
+
+__device__ __forceinline__ float4 cluster_ld4(uint32_t addr) {
+  float4 f;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(addr));
+  return f;
+}
+__device__ __forceinline__ float act_any(int act, float g) {
+  return act == FP4AR_ACT_SILU ? act_value<FP4AR_ACT_SILU>(g) : act == FP4AR_ACT_GELU ? act_value<FP4AR_ACT_GELU>(g) : act_value<FP4AR_ACT_GELU_TANH>(g);
+}
+
+template <int OP>
+__global__ void __launch_bounds__(192, 2)
+few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ FewParams p) {
+  static_assert(OP == kGated || OP == kAdapt, "forward products");
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kFewStagesMax], empty[kFewStagesMax], acc_full;
+  __shared__ uint32_t tmem_holder;
+  __shared__ volatile uint32_t abort_flag;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  float* part = reinterpret_cast<float*>(ring);  // [tokens][128], once the ring has been read
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tile = blockIdx.x / p.split, crank = blockIdx.x % p.split;
+  const int stage_bytes = kOpBytes + p.tokens * 128;
+  const uint32_t cols = p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
+  if (tid == 0) {
+    for (int s = 0; s < p.stages; s++) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
+    mbar_init(&acc_full, 1);
+    abort_flag = 0u;
+    mbar_init_fence();
+    prefetch_tensormap(&map_w);
+    prefetch_tensormap(&map_x);
+  }
+  if (warp == 1) { tmem_alloc(&tmem_holder, cols); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_holder;
+  GemmWait gw{&abort_flag, p.status, p.timeout_ns};
+  // kAdapt: the launch before this one lets it start only after its own wait, so everything before that one is complete here; what
+  // that one itself writes (V) is waited for where it is read.
+  if (OP != kAdapt) pdl_wait_prior_grids();
+  if (OP != kAdapt) pdl_release_dependents();
+
+  const int kb0 = p.kblocks * crank / p.split, kb1 = p.kblocks * (crank + 1) / p.split;
+  const int row0 = OP == kGated ? tile * 64 : tile * 128, row1 = OP == kGated ? p.N + row0 : row0 + 64;
+  int issued = 0;
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int kb = kb0; kb < kb1; kb++, issued++) {
+        const int s = issued % p.stages;
+        if (!gemm_wait(empty + s, ((issued / p.stages) & 1u) ^ 1u, gw, 1)) break;
+        uint8_t* at = ring + s * stage_bytes;
+        mbar_arrive_expect(full + s, stage_bytes);
+        tma_load_2d(at, &map_w, kb * kBlockK, row0, full + s);
+        tma_load_2d(at + kOpBytes / 2, &map_w, kb * kBlockK, row1, full + s);
+        tma_load_2d(at + kOpBytes, &map_x, kb * kBlockK, 0, full + s);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.tokens >> 3) << 17) | ((128u >> 4) << 24);
+      for (int it = 0; it < kb1 - kb0; it++) {
+        const int s = it % p.stages;
+        if (!gemm_wait(full + s, (it / p.stages) & 1u, gw, 3)) break;
+        tc_fence_after();
+        const uint64_t da = umma_desc_k128(ring + s * stage_bytes), db = umma_desc_k128(ring + s * stage_bytes + kOpBytes);
+#pragma unroll
+        for (int k = 0; k < kBlockK / 16; k++) umma_bf16(tmem_base, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (it | k) != 0 ? 1u : 0u);
+        umma_commit(empty + s);
+      }
+      umma_commit(&acc_full);
+    }
+  } else {
+    if constexpr (OP == kAdapt) {
+      // bring the B rows of this CTA's outputs into L2
+      for (int i = crank * 128 + tid - 64; i < p.M * 32; i += p.split * 128) {
+        const int id = p.ids[i / 32], n = row0 + i % 32 * 4;
+        if (id >= 0 && id < p.adapters && n < p.N) {
+          const char* b = reinterpret_cast<const char*>(p.b + ((size_t)id * p.N + n) * p.R);
+          for (int o = 0; o < 8 * p.R; o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
+        }
+      }
+    }
+    const int q = warp & 3;
+    if (__all_sync(0xffffffffu, gemm_wait(&acc_full, 0u, gw, 4)) && !__any_sync(0xffffffffu, abort_flag != 0u)) {
+      tc_fence_after();
+      for (int c = 0; c < p.tokens; c += 16) {
+        float v[16];
+        tmem_ld16_issue(tmem_base + ((uint32_t)(q * 32) << 16) + c, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; i++) part[(c + i) * 128 + q * 32 + lane] = v[i];
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (abort_flag != 0u) {
+    if (tid == 0)
+      for (int i = max(0, issued - p.stages); i < issued; i++) gemm_settle(full + i % p.stages, (i / p.stages) & 1);
+    if (tid == 32) gemm_settle(&acc_full, 0u);       // committed behind every MMA issued
+    __syncthreads();
+  }
+  if (OP == kAdapt) pdl_wait_prior_grids();
+  if (OP == kAdapt) pdl_release_dependents();
+  if (p.split > 1) cluster_sync_all();
+  // Four neighbouring outputs of a row at a time.
+  const uint32_t base = smem_addr(part);
+  auto sum4 = [&](int at) {
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int d = 0; d < p.split; d++) {
+      float4 f;
+      if (p.split > 1) {
+        uint32_t a;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(base + at * 4), "r"(d));
+        f = cluster_ld4(a);
+      } else {
+        f = *reinterpret_cast<const float4*>(part + at);
+      }
+      s.x += f.x; s.y += f.y; s.z += f.z; s.w += f.w;
+    }
+    return s;
+  };
+  if constexpr (OP == kGated) {
+    for (int i = crank * 192 + tid; i < p.M * 16; i += p.split * 192) {
+      const int m = i / 16, c = i % 16 * 4, f = row0 + c;
+      if (f >= p.N) continue;
+      const float4 g = sum4(m * 128 + c), u = sum4(m * 128 + 64 + c);
+      if (p.pre) {
+        *reinterpret_cast<float4*>(p.pre + (size_t)m * 2 * p.N + f) = g;
+        *reinterpret_cast<float4*>(p.pre + ((size_t)m * 2 + 1) * p.N + f) = u;
+      }
+      const uint2 h = make_uint2(pack_bf16(act_any(p.act, g.x) * u.x, act_any(p.act, g.y) * u.y),
+                                 pack_bf16(act_any(p.act, g.z) * u.z, act_any(p.act, g.w) * u.w));
+      *reinterpret_cast<uint2*>(p.out + (size_t)m * p.N + f) = h;
+    }
+  } else {
+    const int line = (p.R + kChunk - 1) / kChunk * 64;
+    for (int i = crank * 192 + tid; i < p.M * 32; i += p.split * 192) {
+      const int m = i / 32, c = i % 32 * 4, n = row0 + c;
+      if (n >= p.N) continue;
+      const int id = p.ids[m];
+      float4 s = sum4(m * 128 + c);
+      if (id >= 0 && id < p.adapters) {
+        const uint4* b = reinterpret_cast<const uint4*>(p.b + ((size_t)id * p.N + n) * p.R);
+        const __nv_bfloat16* v = p.v + (size_t)m * line;
+        float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int r = 0; r < p.R; r += 8) {
+          const uint4 hi = __ldcg(reinterpret_cast<const uint4*>(v + r / kChunk * 64 + r % kChunk));
+          const uint4 lo = __ldcg(reinterpret_cast<const uint4*>(v + r / kChunk * 64 + r % kChunk + kChunk));
+          const uint32_t h4[4] = {hi.x, hi.y, hi.z, hi.w}, l4[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const uint4 w = b[(j * p.R + r) / 8];
+            const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              low[j] = fmaf(bf16_hi(h4[e]) + bf16_hi(l4[e]), bf16_hi(w4[e]), fmaf(bf16_lo(h4[e]) + bf16_lo(l4[e]), bf16_lo(w4[e]), low[j]));
+          }
+        }
+        s.x += low[0]; s.y += low[1]; s.z += low[2]; s.w += low[3];
+      }
+      *reinterpret_cast<uint2*>(p.out + (size_t)m * p.N + n) = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+    }
+  }
+  if (p.split > 1) cluster_sync_all();               // a CTA's sums are read until here
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, cols);
+  }
+}
+
+// `rows` rows of W: 2 N (kGated) or N.
+template <int OP>
+int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p, cudaStream_t stream) {
+  constexpr int kBudget = 110 * 1024;                // of dynamic shared memory: two CTAs an SM
+  static std::atomic<int> raised[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cuda_fail();
+  if (!raised[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(few_rows_kernel<OP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget) != cudaSuccess) return cuda_fail();
+    raised[dev].store(1, std::memory_order_release);
+  }
+  p.status = gemm_status_word();
+  if (!p.status) return cuda_fail();
+  p.timeout_ns = kWaitLimitNs;
+  p.tokens = (p.M + 15) / 16 * 16;
+  p.kblocks = (K + 63) / 64;
+  CUtensorMap mw, mx;
+  if (!map_2d(&mw, w, rows, K, 64) || !map_2d(&mx, x, p.M, K, p.tokens)) return FP4AR_ERR_UNSUPPORTED;
+  const int per_tile = OP == kGated ? 64 : 128, tiles = (p.N + per_tile - 1) / per_tile, slots = 2 * device_sm_count();
+  p.split = 1;
+  while (p.split < 8 && (p.split + 1) * tiles <= slots && 2 * (p.split + 1) <= p.kblocks) p.split++;
+  const int stage = kOpBytes + p.tokens * 128, blocks = (p.kblocks + p.split - 1) / p.split, sums = p.tokens * 512;
+  p.stages = (kBudget - 1024) / stage;
+  if (p.stages > kFewStagesMax) p.stages = kFewStagesMax;
+  if (p.stages > blocks) p.stages = blocks;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(tiles * p.split);
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = (p.stages * stage > sums ? p.stages * stage : sums) + 1024;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.split > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, few_rows_kernel<OP>, mw, mx, p) != cudaSuccess) return cuda_fail();
+  return cuda_check_launch();
+}
+
+}  // namespace layer
+}  // namespace fp4ar

@@ -4,6 +4,7 @@
 // and dW = dpre^T x.  The projections are kept in FP32: in BF16 their rounding doubles the gradients' error (relative to
 // 64 bits 0.0030 instead of 0.0024, where the rounding of the results alone is 0.0017).  dpre is rounded to BF16, the type that
 // the tensor cores take.
+#include "few_rows.cuh"
 #include "layer_gemm.cuh"
 
 namespace fp4ar {
@@ -75,6 +76,12 @@ extern "C" int fp4ar_gated_linear(const void* x, const void* wt, int M, int F, i
   if (!shape_ok(M, F, K, act)) return FP4AR_ERR_ARGUMENT;
   if (M == 0) return FP4AR_OK;
   if (!x || !wt || !h || !aligned16(x, wt, h, pre)) return FP4AR_ERR_ARGUMENT;
+  if (M <= kFewRows) {
+    FewParams fp;
+    memset(&fp, 0, sizeof(fp));
+    fp.M = M; fp.N = F; fp.act = act; fp.out = (__nv_bfloat16*)h; fp.pre = (float*)pre;
+    return launch_few_rows<kGated>(wt, 2L * F, x, K, fp, (cudaStream_t)stream);
+  }
   Maps maps;
   memset(&maps, 0, sizeof(maps));
   if (!map_2d(&maps.a, x, M, K, 128) || !map_2d(&maps.b, wt, 2L * F, K, 128) || !map_2d(&maps.out, h, M, F, 32) ||
