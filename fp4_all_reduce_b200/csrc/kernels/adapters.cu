@@ -291,12 +291,13 @@ __global__ void __launch_bounds__(256) few_low_rank_kernel(const __nv_bfloat16* 
     uint4 xv[8], av[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      const bool in = i + 32 * j < K / 8;
-      av[j] = in ? ldg16(ap + i + 32 * j) : make_uint4(0, 0, 0, 0);
-      xv[j] = in ? ldg16(xp + i + 32 * j) : make_uint4(0, 0, 0, 0);
+      const int at = min(i + 32 * j, K / 8 - 1);
+      av[j] = ldg16(ap + at);
+      xv[j] = ldg16(xp + at);
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) {
+      if (i + 32 * j >= K / 8) xv[j] = make_uint4(0, 0, 0, 0), av[j] = make_uint4(0, 0, 0, 0);
       const uint32_t xw[4] = {xv[j].x, xv[j].y, xv[j].z, xv[j].w}, aw[4] = {av[j].x, av[j].y, av[j].z, av[j].w};
 #pragma unroll
       for (int e = 0; e < 4; e++) s = fmaf(bf16_hi(xw[e]), bf16_hi(aw[e]), fmaf(bf16_lo(xw[e]), bf16_lo(aw[e]), s));

@@ -5,8 +5,8 @@
 // a long chain of K blocks, so a cluster of up to eight CTAs cuts K: each leaves its FP32 sums in shared memory, and all of them add
 // up a share of the outputs, in the order of the CTAs.  Two CTAs fit an SM, one's set-up and sums run under the other's loads.
 //   kGated   the 128 rows are 64 gate rows and the 64 up rows that go with them: their product is taken where the sums meet
-//   kAdapt   the low-rank part of an output is added there too, by plain FP32 products with V.  V comes from a launch before this
-//            one; only that step waits for it (see below), the weights are on their way meanwhile
+//   kAdapt   the low-rank parts of the outputs that a CTA adds up are computed by the epilogue warps while the weights stream in, by
+//            plain FP32 products with V.  V comes from a launch before this one; only those warps wait for it (see below)
 #pragma once
 #include "layer_gemm.cuh"
 
@@ -21,7 +21,7 @@ struct FewParams {
   __nv_bfloat16* out;
   float* pre;                                    // kGated, optional [M][2 N]
   // kAdapt, as in Params
-  int R, adapters;
+  int R, adapters, low_offset;
   const int* ids;
   const __nv_bfloat16* v;
   const __nv_bfloat16* b;
@@ -51,7 +51,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tile = blockIdx.x / p.split, crank = blockIdx.x % p.split;
   const int stage_bytes = kOpBytes + p.tokens * 128;
-  const uint32_t cols = p.tokens <= 32 ? 32 : p.tokens <= 64 ? 64 : 128;
+  constexpr uint32_t cols = 128;
   if (tid == 0) {
     for (int s = 0; s < p.stages; s++) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
     mbar_init(&acc_full, 1);
@@ -69,10 +69,13 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   // kAdapt: the launch before this one lets it start only after its own wait, so everything before that one is complete here; what
   // that one itself writes (V) is waited for where it is read.
   if (OP != kAdapt) pdl_wait_prior_grids();
-  if (OP != kAdapt) pdl_release_dependents();
+  pdl_release_dependents();
 
   const int kb0 = p.kblocks * crank / p.split, kb1 = p.kblocks * (crank + 1) / p.split;
   const int row0 = OP == kGated ? tile * 64 : tile * 128, row1 = OP == kGated ? p.N + row0 : row0 + 64;
+  // this CTA's share of the outputs, in groups of four
+  const int items = p.M * (OP == kGated ? 16 : 32), item0 = items * crank / p.split, item1 = items * (crank + 1) / p.split;
+  float4* lows = reinterpret_cast<float4*>(ring + p.low_offset);
   int issued = 0;
   if (warp == 0) {
     if (lane == 0) {
@@ -102,13 +105,49 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
   } else {
     if constexpr (OP == kAdapt) {
-      // bring the B rows of this CTA's outputs into L2
-      for (int i = crank * 128 + tid - 64; i < p.M * 32; i += p.split * 128) {
-        const int id = p.ids[i / 32], n = row0 + i % 32 * 4;
-        if (id >= 0 && id < p.adapters && n < p.N) {
-          const char* b = reinterpret_cast<const char*>(p.b + ((size_t)id * p.N + n) * p.R);
+      // the low-rank parts of this CTA's share of the outputs, four of a row at a time; their B rows are asked for before V is there
+      auto b_rows = [&](int i, int& m, int& n) -> const uint4* {
+        m = i / 32;
+        n = row0 + i % 32 * 4;
+        const int id = p.ids[m];
+        return id >= 0 && id < p.adapters && n < p.N ? reinterpret_cast<const uint4*>(p.b + ((size_t)id * p.N + n) * p.R) : nullptr;
+      };
+      int m, n;
+      for (int i = item0 + tid - 64; i < item1; i += 128)
+        if (const char* b = reinterpret_cast<const char*>(b_rows(i, m, n)))
           for (int o = 0; o < 8 * p.R; o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
+      pdl_wait_prior_grids();
+      for (int i = item0 + tid - 64; i < item1; i += 128) {
+        float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (const uint4* b = b_rows(i, m, n)) {
+          const __nv_bfloat16* v = p.v + (size_t)m * ((p.R + kChunk - 1) / kChunk * 64);
+          // sixteen ranks at a time, their twelve loads in flight together (past the last rank: the last eight again, not added)
+          for (int r = 0; r < p.R; r += 16) {
+            uint4 hi[2], lo[2], w[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const int at = min(r + 8 * h, p.R - 8);
+              const uint4* line = reinterpret_cast<const uint4*>(v + at / kChunk * 64 + at % kChunk);
+              hi[h] = __ldcg(line);
+              lo[h] = __ldcg(line + kChunk / 8);
+#pragma unroll
+              for (int j = 0; j < 4; j++) w[h][j] = __ldg(b + (j * p.R + at) / 8);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              if (r + 8 * h >= p.R) break;
+              const uint32_t h4[4] = {hi[h].x, hi[h].y, hi[h].z, hi[h].w}, l4[4] = {lo[h].x, lo[h].y, lo[h].z, lo[h].w};
+#pragma unroll
+              for (int j = 0; j < 4; j++) {
+                const uint32_t w4[4] = {w[h][j].x, w[h][j].y, w[h][j].z, w[h][j].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  low[j] = fmaf(bf16_hi(h4[e]) + bf16_hi(l4[e]), bf16_hi(w4[e]), fmaf(bf16_lo(h4[e]) + bf16_lo(l4[e]), bf16_lo(w4[e]), low[j]));
+              }
+            }
+          }
         }
+        lows[i - item0] = make_float4(low[0], low[1], low[2], low[3]);
       }
     }
     const int q = warp & 3;
@@ -132,8 +171,6 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (tid == 32) gemm_settle(&acc_full, 0u);       // committed behind every MMA issued
     __syncthreads();
   }
-  if (OP == kAdapt) pdl_wait_prior_grids();
-  if (OP == kAdapt) pdl_release_dependents();
   if (p.split > 1) cluster_sync_all();
   // Four neighbouring outputs of a row at a time.
   const uint32_t base = smem_addr(part);
@@ -153,7 +190,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     return s;
   };
   if constexpr (OP == kGated) {
-    for (int i = crank * 192 + tid; i < p.M * 16; i += p.split * 192) {
+    for (int i = item0 + tid; i < item1; i += 192) {
       const int m = i / 16, c = i % 16 * 4, f = row0 + c;
       if (f >= p.N) continue;
       const float4 g = sum4(m * 128 + c), u = sum4(m * 128 + 64 + c);
@@ -166,32 +203,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       *reinterpret_cast<uint2*>(p.out + (size_t)m * p.N + f) = h;
     }
   } else {
-    const int line = (p.R + kChunk - 1) / kChunk * 64;
-    for (int i = crank * 192 + tid; i < p.M * 32; i += p.split * 192) {
+    for (int i = item0 + tid; i < item1; i += 192) {
       const int m = i / 32, c = i % 32 * 4, n = row0 + c;
       if (n >= p.N) continue;
-      const int id = p.ids[m];
-      float4 s = sum4(m * 128 + c);
-      if (id >= 0 && id < p.adapters) {
-        const uint4* b = reinterpret_cast<const uint4*>(p.b + ((size_t)id * p.N + n) * p.R);
-        const __nv_bfloat16* v = p.v + (size_t)m * line;
-        float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int r = 0; r < p.R; r += 8) {
-          const uint4 hi = __ldcg(reinterpret_cast<const uint4*>(v + r / kChunk * 64 + r % kChunk));
-          const uint4 lo = __ldcg(reinterpret_cast<const uint4*>(v + r / kChunk * 64 + r % kChunk + kChunk));
-          const uint32_t h4[4] = {hi.x, hi.y, hi.z, hi.w}, l4[4] = {lo.x, lo.y, lo.z, lo.w};
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const uint4 w = b[(j * p.R + r) / 8];
-            const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              low[j] = fmaf(bf16_hi(h4[e]) + bf16_hi(l4[e]), bf16_hi(w4[e]), fmaf(bf16_lo(h4[e]) + bf16_lo(l4[e]), bf16_lo(w4[e]), low[j]));
-          }
-        }
-        s.x += low[0]; s.y += low[1]; s.z += low[2]; s.w += low[3];
-      }
-      *reinterpret_cast<uint2*>(p.out + (size_t)m * p.N + n) = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+      const float4 s = sum4(m * 128 + c), low = lows[i - item0];
+      *reinterpret_cast<uint2*>(p.out + (size_t)m * p.N + n) = make_uint2(pack_bf16(s.x + low.x, s.y + low.y), pack_bf16(s.z + low.z, s.w + low.w));
     }
   }
   if (p.split > 1) cluster_sync_all();               // a CTA's sums are read until here
@@ -202,6 +218,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   }
 }
 
+// Stands in for few_rows_kernel where the runtime is asked how many clusters fit: for a kernel that allocates TMEM it answers with one CTA
+// an SM whatever the kernel takes (two were seen to run side by side).
+template <int OP>
+__global__ void __launch_bounds__(192, 2) few_rows_room_kernel() {}
+
 // `rows` rows of W: 2 N (kGated) or N.
 template <int OP>
 int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p, cudaStream_t stream) {
@@ -209,8 +230,27 @@ int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p,
   static std::atomic<int> raised[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cuda_fail();
+  static std::atomic<int> clusters[64][9];           // how many clusters of a size can be resident
   if (!raised[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(few_rows_kernel<OP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget) != cudaSuccess) return cuda_fail();
+    if (cudaFuncSetAttribute(few_rows_kernel<OP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget) != cudaSuccess ||
+        cudaFuncSetAttribute(few_rows_kernel<OP>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
+        cudaFuncSetAttribute(few_rows_room_kernel<OP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget + 1024) != cudaSuccess)
+      return cuda_fail();
+    for (int c = 2; c <= 8; c++) {
+      cudaLaunchConfig_t cfg;
+      memset(&cfg, 0, sizeof(cfg));
+      cfg.gridDim = dim3(64 * c);
+      cfg.blockDim = dim3(192);
+      cfg.dynamicSmemBytes = kBudget + 256;          // and the barriers
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = c; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, few_rows_room_kernel<OP>, &cfg) != cudaSuccess) return cuda_fail();
+      clusters[dev][c].store(n, std::memory_order_release);
+    }
     raised[dev].store(1, std::memory_order_release);
   }
   p.status = gemm_status_word();
@@ -220,18 +260,22 @@ int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p,
   p.kblocks = (K + 63) / 64;
   CUtensorMap mw, mx;
   if (!map_2d(&mw, w, rows, K, 64) || !map_2d(&mx, x, p.M, K, p.tokens)) return FP4AR_ERR_UNSUPPORTED;
-  const int per_tile = OP == kGated ? 64 : 128, tiles = (p.N + per_tile - 1) / per_tile, slots = 2 * device_sm_count();
+  const int per_tile = OP == kGated ? 64 : 128, tiles = (p.N + per_tile - 1) / per_tile;
+  // the widest split whose clusters are all resident at once (of six CTAs 45 fit, not 49: a cluster stays within a part of the GPU)
   p.split = 1;
-  while (p.split < 8 && (p.split + 1) * tiles <= slots && 2 * (p.split + 1) <= p.kblocks) p.split++;
+  for (int c = 2; c <= 8 && 2 * c <= p.kblocks; c++)
+    if (tiles <= clusters[dev][c].load(std::memory_order_acquire)) p.split = c;
   const int stage = kOpBytes + p.tokens * 128, blocks = (p.kblocks + p.split - 1) / p.split, sums = p.tokens * 512;
-  p.stages = (kBudget - 1024) / stage;
+  const int lows = OP == kAdapt ? ((p.M * 32 + p.split - 1) / p.split + 1) * 16 : 0;
+  p.stages = (kBudget - 1024 - lows) / stage;
   if (p.stages > kFewStagesMax) p.stages = kFewStagesMax;
   if (p.stages > blocks) p.stages = blocks;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(tiles * p.split);
   cfg.blockDim = dim3(192);
-  cfg.dynamicSmemBytes = (p.stages * stage > sums ? p.stages * stage : sums) + 1024;
+  p.low_offset = p.stages * stage > sums ? p.stages * stage : sums;
+  cfg.dynamicSmemBytes = p.low_offset + lows + 1024;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -19,6 +19,8 @@
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 #include <torch/library.h>
@@ -300,6 +302,31 @@ std::tuple<Tensor, Tensor> op_gated_backward(const Tensor& dh, const Tensor& pre
   return {std::move(dx), std::move(dw)};
 }
 
+// Records h for autograd.  (As a Python function the forward and backward pass cost 25 us more of host time than the launches, and the
+// backward pass took the interpreter's lock.)
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& wt, int64_t act) {
+    auto r = op_gated_linear(x, wt, act, true, Tensor());
+    ctx->save_for_backward({x, wt, std::get<1>(r)});
+    ctx->saved_data["activation"] = act;
+    return std::get<0>(r);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    auto r = op_gated_backward(grads[0].contiguous(), saved[2], saved[0], saved[1], ctx->saved_data["activation"].toInt(), ctx->needs_input_grad(0),
+                               ctx->needs_input_grad(1));
+    torch::autograd::variable_list out{std::move(std::get<0>(r)), std::move(std::get<1>(r))};
+    if (at::GradMode::is_enabled()) {            // create_graph: the gradients cannot be differentiated again, and say so
+      for (Tensor& t : out)
+        if (t.defined()) t = t.detach().set_requires_grad(true);
+      out = (*std::make_shared<torch::autograd::DelayedError>("gated_linear cannot be differentiated twice", 2))(std::move(out));
+    }
+    out.emplace_back();
+    return out;
+  }
+};
+Tensor op_gated_linear_recorded(const Tensor& x, const Tensor& wt, int64_t act) { return GatedLinear::apply(x, wt, act); }
+
 Tensor op_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, const Tensor& a, const Tensor& b, const Tensor& scales, Tensor out) {
   TORCH_CHECK_VALUE(x.dim() == 2, "x must have shape [rows, K], got ", shape_text(x));
   TORCH_CHECK_VALUE(wt.dim() == 2 && wt.size(1) == x.size(1), "wt must have shape [N, ", x.size(1), "], got ", shape_text(wt));
@@ -503,6 +530,15 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return wrap2_or_none([&] { NoGil g; return op_gated_linear(x, wt, act, pre, std::move(out)); }());
   END_HANDLE_TH_ERRORS
 }
+// (x, wt, activation): h, recorded for autograd
+PyObject* py_gated_linear_recorded(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arity(n, 3);
+  const Tensor &x = tensor_arg(a[0], "x"), &wt = tensor_arg(a[1], "wt");
+  const int64_t act = int_arg(a[2]);
+  return THPVariable_Wrap([&] { NoGil g; return op_gated_linear_recorded(x, wt, act); }());
+  END_HANDLE_TH_ERRORS
+}
 // (dh, pre, x, wt, activation, need_dx, need_dw): (dx or None, dwt or None)
 PyObject* py_gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -688,7 +724,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FP4AR_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FP4AR_METHOD(bind), FP4AR_METHOD(encode), FP4AR_METHOD(encode_static), FP4AR_METHOD(decode_sum),
-                         FP4AR_METHOD(reduce_reencode), FP4AR_METHOD(add_rmsnorm), FP4AR_METHOD(gemm), FP4AR_METHOD(gated_linear), FP4AR_METHOD(gated_backward),
+                         FP4AR_METHOD(reduce_reencode), FP4AR_METHOD(add_rmsnorm), FP4AR_METHOD(gemm), FP4AR_METHOD(gated_linear), FP4AR_METHOD(gated_linear_recorded), FP4AR_METHOD(gated_backward),
                          FP4AR_METHOD(linear_adapters), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fp4ar_front", nullptr, -1, methods};
 

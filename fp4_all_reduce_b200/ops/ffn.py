@@ -18,27 +18,10 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native as N
 
 ACTIVATIONS = {"silu": N.ACT_SILU, "gelu": N.ACT_GELU, "gelu_tanh": N.ACT_GELU_TANH}
-
-
-class _GatedLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, wt, activation):
-        h, pre = N.front().gated_linear(x, wt, activation, True, None)
-        ctx.save_for_backward(x, wt, pre)
-        ctx.activation = activation
-        return h
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh):
-        x, wt, pre = ctx.saved_tensors
-        dx, dwt = gated_linear_backward(dh, pre, x, wt, ctx.activation, need_dx=ctx.needs_input_grad[0], need_dwt=ctx.needs_input_grad[1])
-        return dx, dwt, None
 
 
 def gated_linear(x: torch.Tensor, wt: torch.Tensor, activation: int = N.ACT_SILU, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -47,7 +30,7 @@ def gated_linear(x: torch.Tensor, wt: torch.Tensor, activation: int = N.ACT_SILU
     if torch.is_grad_enabled() and (x.requires_grad or wt.requires_grad):
         if out is not None:
             raise ValueError("out cannot be given where a gradient is recorded")
-        return _GatedLinear.apply(x, wt, activation)
+        return N.front().gated_linear_recorded(x, wt, activation)
     return N.front().gated_linear(x, wt, activation, False, out)[0]
 
 
