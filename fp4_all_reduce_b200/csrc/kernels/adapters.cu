@@ -276,7 +276,7 @@ __device__ __forceinline__ uint4 ldg16(const uint4* p) {      // volatile: issue
 
 // V of few rows: eight ranks of a row per CTA, a warp for each.  Bound by latency: a row of A_a is K numbers, eight loads of every lane in
 // flight.
-__global__ void __launch_bounds__(256) few_low_rank_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ a,
+__global__ void __launch_bounds__(256, 3) few_low_rank_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ a,
                                                            const int* __restrict__ ids, const float* __restrict__ scales, int K, int R, int adapters,
                                                            __nv_bfloat16* __restrict__ v) {
   pdl_wait_prior_grids();

@@ -105,49 +105,63 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
   } else {
     if constexpr (OP == kAdapt) {
-      // the low-rank parts of this CTA's share of the outputs, four of a row at a time; their B rows are asked for before V is there
-      auto b_rows = [&](int i, int& m, int& n) -> const uint4* {
-        m = i / 32;
-        n = row0 + i % 32 * 4;
+      // The low-rank parts of this CTA's share of the outputs, a warp for each row of x.  B_a is read as it lies: `width` lanes have 16
+      // bytes each of one of its rows (eight ranks, whose V stay in registers), so a warp's load is 512 contiguous bytes, and the
+      // lanes of a row add up by shuffles.  (A lane with four rows of its own: 41 us instead of 5 at 64 rows, R = 64.)  The lines
+      // are asked for before V is there.
+      const int pieces = p.R / 8, width = pieces > 8 ? 16 : pieces > 4 ? 8 : pieces > 2 ? 4 : pieces, per_load = 32 / width;
+      const int sub = lane % width, line = (p.R + kChunk - 1) / kChunk * 64;
+      auto share_of = [&](int m, int& from, int& to) -> const uint4* {      // B_a from row `row0` on, rows [from, to) of the tile
+        from = max(4 * item0 - m * 128, 0);
+        to = min(min(4 * item1 - m * 128, 128), p.N - row0);
         const int id = p.ids[m];
-        return id >= 0 && id < p.adapters && n < p.N ? reinterpret_cast<const uint4*>(p.b + ((size_t)id * p.N + n) * p.R) : nullptr;
+        return id >= 0 && id < p.adapters ? reinterpret_cast<const uint4*>(p.b + ((size_t)id * p.N + row0) * p.R) : nullptr;
       };
-      int m, n;
-      for (int i = item0 + tid - 64; i < item1; i += 128)
-        if (const char* b = reinterpret_cast<const char*>(b_rows(i, m, n)))
-          for (int o = 0; o < 8 * p.R; o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
+      const int m0 = item0 / 32 + warp - 2, m1 = (item1 + 31) / 32;
+      int from, to;
+      for (int m = m0; m < m1; m += 4)
+        if (const uint4* b = share_of(m, from, to))
+          for (int o = from * pieces + lane * 8; o < to * pieces; o += 32 * 8) asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
       pdl_wait_prior_grids();
-      for (int i = item0 + tid - 64; i < item1; i += 128) {
-        float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (const uint4* b = b_rows(i, m, n)) {
-          const __nv_bfloat16* v = p.v + (size_t)m * ((p.R + kChunk - 1) / kChunk * 64);
-          // sixteen ranks at a time, their twelve loads in flight together (past the last rank: the last eight again, not added)
-          for (int r = 0; r < p.R; r += 16) {
-            uint4 hi[2], lo[2], w[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const int at = min(r + 8 * h, p.R - 8);
-              const uint4* line = reinterpret_cast<const uint4*>(v + at / kChunk * 64 + at % kChunk);
-              hi[h] = __ldcg(line);
-              lo[h] = __ldcg(line + kChunk / 8);
-#pragma unroll
-              for (int j = 0; j < 4; j++) w[h][j] = __ldg(b + (j * p.R + at) / 8);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              if (r + 8 * h >= p.R) break;
-              const uint32_t h4[4] = {hi[h].x, hi[h].y, hi[h].z, hi[h].w}, l4[4] = {lo[h].x, lo[h].y, lo[h].z, lo[h].w};
-#pragma unroll
-              for (int j = 0; j < 4; j++) {
-                const uint32_t w4[4] = {w[h][j].x, w[h][j].y, w[h][j].z, w[h][j].w};
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                  low[j] = fmaf(bf16_hi(h4[e]) + bf16_hi(l4[e]), bf16_hi(w4[e]), fmaf(bf16_lo(h4[e]) + bf16_lo(l4[e]), bf16_lo(w4[e]), low[j]));
-              }
-            }
-          }
+      for (int m = m0; m < m1; m += 4) {
+        const uint4* b = share_of(m, from, to);
+        float* low = reinterpret_cast<float*>(lows) + m * 128 - 4 * item0;
+        if (!b) {
+          for (int r = from + lane; r < to; r += 32) low[r] = 0.0f;
+          continue;
         }
-        lows[i - item0] = make_float4(low[0], low[1], low[2], low[3]);
+        float v[8];
+        const int piece = min(sub, pieces - 1);          // (lanes beyond the last piece read it too and add nothing)
+        const uint4* at = reinterpret_cast<const uint4*>(p.v + (size_t)m * line + piece / 4 * 64 + piece % 4 * 8);
+        const uint4 hi = __ldcg(at), lo = __ldcg(at + kChunk / 8);
+        const uint32_t h4[4] = {hi.x, hi.y, hi.z, hi.w}, l4[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          v[2 * e] = bf16_lo(h4[e]) + bf16_lo(l4[e]);
+          v[2 * e + 1] = bf16_hi(h4[e]) + bf16_hi(l4[e]);
+        }
+        for (int r0 = from; r0 < to; r0 += 8 * per_load) {                                   // eight loads in flight
+          const int r = r0 + lane / width;
+          uint4 w[8];
+          float s[8];
+#pragma unroll
+          for (int k = 0; k < 8; k++) w[k] = __ldg(b + min(r + k * per_load, to - 1) * pieces + piece);
+#pragma unroll
+          for (int k = 0; k < 8; k++) {
+            const uint32_t w4[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+            s[k] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[k] = fmaf(v[2 * e + 1], bf16_hi(w4[e]), fmaf(v[2 * e], bf16_lo(w4[e]), s[k]));
+            if (sub >= pieces) s[k] = 0.0f;
+          }
+          for (int o = width / 2; o; o >>= 1) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+          }
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if (sub == 0 && r + k * per_load < to) low[r + k * per_load] = s[k];
+        }
       }
     }
     const int q = warp & 3;
