@@ -341,7 +341,7 @@ extern "C" int fp4ar_linear_adapters(const void* x, const void* wt, const int* i
     return FP4AR_ERR_ARGUMENT;
   const cudaStream_t stream = (cudaStream_t)stream_;
   const Workspace ws(workspace, M, R);
-  if (M <= kFewRows) {
+  if (M <= kNarrowRows) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(M, R / 8);
@@ -358,7 +358,7 @@ extern "C" int fp4ar_linear_adapters(const void* x, const void* wt, const int* i
     memset(&fp, 0, sizeof(fp));
     fp.M = M; fp.N = N; fp.out = (__nv_bfloat16*)y;
     fp.R = R; fp.adapters = adapters; fp.ids = ids; fp.v = ws.v; fp.b = (const __nv_bfloat16*)b;
-    return launch_few_rows<kAdapt>(wt, N, x, K, fp, stream);
+    return launch_few_rows<kAdapt, false>(wt, N, x, K, fp, stream);
   }
   LowParams lp;
   memset(&lp, 0, sizeof(lp));

@@ -1,9 +1,10 @@
-// The same products for few rows (M <= 128), where the time is that of reading the weights once.
+// The same products for few rows, where the time is that of reading the weights once.
 //
-// The operands change sides: 128 rows of W are the M of the tcgen05 product and the rows of x its N (16 .. 128), so nothing is
-// multiplied for rows that are not there.  A CTA of its own for every 128 rows of W would leave SMs idle and the others with
-// a long chain of K blocks, so a cluster of up to eight CTAs cuts K: each leaves its FP32 sums in shared memory, and all of them add
-// up a share of the outputs, in the order of the CTAs.  Two CTAs fit an SM, one's set-up and sums run under the other's loads.
+// The operands change sides: 128 rows of W (kInput: columns) are the M of the tcgen05 product and the rows of x its N (16 .. 256), so
+// next to nothing is multiplied for rows that are not there.  A CTA of its own for every 128 rows of W would leave SMs idle and the
+// others with a long chain of K blocks, so a cluster of up to eight CTAs cuts K: each leaves its FP32 sums in shared memory, and all
+// of them add up a share of the outputs, in the order of the CTAs.  Up to 128 rows two CTAs fit an SM, and one's set-up and sums run
+// under the other's loads (WIDE = false); more rows take groups of up to 256, a CTA for each (WIDE).
 //   kGated   the 128 rows are 64 gate rows and the 64 up rows that go with them: their product is taken where the sums meet
 //   kAdapt   the low-rank parts of the outputs that a CTA adds up are computed by the epilogue warps while the weights stream in, by
 //            plain FP32 products with V.  V comes from a launch before this one; only those warps wait for it (see below)
@@ -13,10 +14,10 @@
 namespace fp4ar {
 namespace layer {
 
-constexpr int kFewRows = 128, kFewStagesMax = 8;
+constexpr int kNarrowRows = 128, kFewStagesMax = 8;
 
 struct FewParams {
-  int M, N, kblocks, split, stages, tokens;      // tokens: M rounded up to 16; N: columns of the output
+  int M, N, kblocks, split, stages, tokens, groups;      // tokens: rows of a group, a multiple of 16; N: columns of the output
   int act;
   __nv_bfloat16* out;
   float* pre;                                    // kGated, optional [M][2 N]
@@ -38,10 +39,10 @@ __device__ __forceinline__ float act_any(int act, float g) {
   return act == FP4AR_ACT_SILU ? act_value<FP4AR_ACT_SILU>(g) : act == FP4AR_ACT_GELU ? act_value<FP4AR_ACT_GELU>(g) : act_value<FP4AR_ACT_GELU_TANH>(g);
 }
 
-template <int OP>
-__global__ void __launch_bounds__(192, 2)
+template <int OP, bool WIDE>
+__global__ void __launch_bounds__(192, WIDE ? 1 : 2)
 few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ FewParams p) {
-  static_assert(OP == kGated || OP == kAdapt, "forward products");
+  static_assert(OP == kGated || OP == kInput || (OP == kAdapt && !WIDE), "products with W");
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kFewStagesMax], empty[kFewStagesMax], acc_full;
   __shared__ uint32_t tmem_holder;
@@ -49,9 +50,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* part = reinterpret_cast<float*>(ring);  // [tokens][128], once the ring has been read
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int tile = blockIdx.x / p.split, crank = blockIdx.x % p.split;
+  // the groups of one tile are neighbours: its weights cross HBM once
+  const int crank = blockIdx.x % p.split, group = blockIdx.x / p.split % p.groups, tile = blockIdx.x / p.split / p.groups;
+  const int first = group * p.tokens, rows = min(p.tokens, p.M - first);
   const int stage_bytes = kOpBytes + p.tokens * 128;
-  constexpr uint32_t cols = 128;
+  constexpr uint32_t cols = WIDE ? 256 : 128;
   if (tid == 0) {
     for (int s = 0; s < p.stages; s++) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
     mbar_init(&acc_full, 1);
@@ -74,7 +77,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   const int kb0 = p.kblocks * crank / p.split, kb1 = p.kblocks * (crank + 1) / p.split;
   const int row0 = OP == kGated ? tile * 64 : tile * 128, row1 = OP == kGated ? p.N + row0 : row0 + 64;
   // this CTA's share of the outputs, in groups of four
-  const int items = p.M * (OP == kGated ? 16 : 32), item0 = items * crank / p.split, item1 = items * (crank + 1) / p.split;
+  const int items = rows * (OP == kGated ? 16 : 32), item0 = items * crank / p.split, item1 = items * (crank + 1) / p.split;
   float4* lows = reinterpret_cast<float4*>(ring + p.low_offset);
   int issued = 0;
   if (warp == 0) {
@@ -84,21 +87,27 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (!gemm_wait(empty + s, ((issued / p.stages) & 1u) ^ 1u, gw, 1)) break;
         uint8_t* at = ring + s * stage_bytes;
         mbar_arrive_expect(full + s, stage_bytes);
-        tma_load_2d(at, &map_w, kb * kBlockK, row0, full + s);
-        tma_load_2d(at + kOpBytes / 2, &map_w, kb * kBlockK, row1, full + s);
-        tma_load_2d(at + kOpBytes, &map_x, kb * kBlockK, 0, full + s);
+        if constexpr (OP == kInput) {
+          tma_load_2d(at, &map_w, row0, kb * kBlockK, full + s);
+          tma_load_2d(at + kOpBytes / 2, &map_w, row1, kb * kBlockK, full + s);
+        } else {
+          tma_load_2d(at, &map_w, kb * kBlockK, row0, full + s);
+          tma_load_2d(at + kOpBytes / 2, &map_w, kb * kBlockK, row1, full + s);
+        }
+        tma_load_2d(at + kOpBytes, &map_x, kb * kBlockK, first, full + s);
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.tokens >> 3) << 17) | ((128u >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((OP == kInput ? 1u : 0u) << 15) | ((uint32_t)(p.tokens >> 3) << 17) | ((128u >> 4) << 24);
       for (int it = 0; it < kb1 - kb0; it++) {
         const int s = it % p.stages;
         if (!gemm_wait(full + s, (it / p.stages) & 1u, gw, 3)) break;
         tc_fence_after();
-        const uint64_t da = umma_desc_k128(ring + s * stage_bytes), db = umma_desc_k128(ring + s * stage_bytes + kOpBytes);
+        const uint8_t* sw = ring + s * stage_bytes;
+        const uint64_t da = OP == kInput ? umma_desc_mn128(sw) : umma_desc_k128(sw), db = umma_desc_k128(ring + s * stage_bytes + kOpBytes);
 #pragma unroll
-        for (int k = 0; k < kBlockK / 16; k++) umma_bf16(tmem_base, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, (it | k) != 0 ? 1u : 0u);
+        for (int k = 0; k < kBlockK / 16; k++) umma_bf16(tmem_base, da + (uint64_t)((OP == kInput ? 128 : 2) * k), db + (uint64_t)(2 * k), idesc, (it | k) != 0 ? 1u : 0u);
         umma_commit(empty + s);
       }
       umma_commit(&acc_full);
@@ -205,9 +214,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   };
   if constexpr (OP == kGated) {
     for (int i = item0 + tid; i < item1; i += 192) {
-      const int m = i / 16, c = i % 16 * 4, f = row0 + c;
+      const int c = i % 16 * 4, f = row0 + c;
       if (f >= p.N) continue;
-      const float4 g = sum4(m * 128 + c), u = sum4(m * 128 + 64 + c);
+      const float4 g = sum4(i / 16 * 128 + c), u = sum4(i / 16 * 128 + 64 + c);
+      const int m = first + i / 16;
       if (p.pre) {
         *reinterpret_cast<float4*>(p.pre + (size_t)m * 2 * p.N + f) = g;
         *reinterpret_cast<float4*>(p.pre + ((size_t)m * 2 + 1) * p.N + f) = u;
@@ -218,10 +228,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
   } else {
     for (int i = item0 + tid; i < item1; i += 192) {
-      const int m = i / 32, c = i % 32 * 4, n = row0 + c;
+      const int c = i % 32 * 4, n = row0 + c;
       if (n >= p.N) continue;
-      const float4 s = sum4(m * 128 + c), low = lows[i - item0];
-      *reinterpret_cast<uint2*>(p.out + (size_t)m * p.N + n) = make_uint2(pack_bf16(s.x + low.x, s.y + low.y), pack_bf16(s.z + low.z, s.w + low.w));
+      const float4 s = sum4(i / 32 * 128 + c), low = OP == kAdapt ? lows[i - item0] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      *reinterpret_cast<uint2*>(p.out + (size_t)(first + i / 32) * p.N + n) = make_uint2(pack_bf16(s.x + low.x, s.y + low.y), pack_bf16(s.z + low.z, s.w + low.w));
     }
   }
   if (p.split > 1) cluster_sync_all();               // a CTA's sums are read until here
@@ -234,23 +244,23 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
 // Stands in for few_rows_kernel where the runtime is asked how many clusters fit: for a kernel that allocates TMEM it answers with one CTA
 // an SM whatever the kernel takes (two were seen to run side by side).
-template <int OP>
-__global__ void __launch_bounds__(192, 2) few_rows_room_kernel() {}
+template <int OP, bool WIDE>
+__global__ void __launch_bounds__(192, WIDE ? 1 : 2) few_rows_room_kernel() {}
 
-// `rows` rows of W: 2 N (kGated) or N.
-template <int OP>
+// `w` has `rows` rows: 2 N of K columns (kGated), N (kAdapt), K rows of N columns (kInput).
+template <int OP, bool WIDE>
 int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p, cudaStream_t stream) {
-  constexpr int kBudget = 110 * 1024;                // of dynamic shared memory: two CTAs an SM
+  constexpr int kBudget = (WIDE ? 220 : 110) * 1024;  // of dynamic shared memory
   static std::atomic<int> raised[64];
+  static std::atomic<int> clusters[64][9];           // how many clusters of a size can be resident
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cuda_fail();
-  static std::atomic<int> clusters[64][9];           // how many clusters of a size can be resident
   if (!raised[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(few_rows_kernel<OP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget) != cudaSuccess ||
-        cudaFuncSetAttribute(few_rows_kernel<OP>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
-        cudaFuncSetAttribute(few_rows_room_kernel<OP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget + 1024) != cudaSuccess)
+    if (cudaFuncSetAttribute(few_rows_kernel<OP, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget) != cudaSuccess ||
+        cudaFuncSetAttribute(few_rows_kernel<OP, WIDE>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
+        cudaFuncSetAttribute(few_rows_room_kernel<OP, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBudget + 1024) != cudaSuccess)
       return cuda_fail();
-    for (int c = 2; c <= 8; c++) {
+    for (int c = 1; c <= 8; c++) {
       cudaLaunchConfig_t cfg;
       memset(&cfg, 0, sizeof(cfg));
       cfg.gridDim = dim3(64 * c);
@@ -262,7 +272,7 @@ int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p,
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, few_rows_room_kernel<OP>, &cfg) != cudaSuccess) return cuda_fail();
+      if (cudaOccupancyMaxActiveClusters(&n, few_rows_room_kernel<OP, WIDE>, &cfg) != cudaSuccess) return cuda_fail();
       clusters[dev][c].store(n, std::memory_order_release);
     }
     raised[dev].store(1, std::memory_order_release);
@@ -270,11 +280,12 @@ int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p,
   p.status = gemm_status_word();
   if (!p.status) return cuda_fail();
   p.timeout_ns = kWaitLimitNs;
-  p.tokens = (p.M + 15) / 16 * 16;
+  p.groups = WIDE ? (p.M + 255) / 256 : 1;
+  p.tokens = ((p.M + p.groups - 1) / p.groups + 15) / 16 * 16;
   p.kblocks = (K + 63) / 64;
   CUtensorMap mw, mx;
-  if (!map_2d(&mw, w, rows, K, 64) || !map_2d(&mx, x, p.M, K, p.tokens)) return FP4AR_ERR_UNSUPPORTED;
-  const int per_tile = OP == kGated ? 64 : 128, tiles = (p.N + per_tile - 1) / per_tile;
+  if (!map_2d(&mw, w, rows, OP == kInput ? p.N : K, 64) || !map_2d(&mx, x, p.M, K, p.tokens)) return FP4AR_ERR_UNSUPPORTED;
+  const int per_tile = OP == kGated ? 64 : 128, tiles = (p.N + per_tile - 1) / per_tile * p.groups;
   // the widest split whose clusters are all resident at once (of six CTAs 45 fit, not 49: a cluster stays within a part of the GPU)
   p.split = 1;
   for (int c = 2; c <= 8 && 2 * c <= p.kblocks; c++)
@@ -298,7 +309,7 @@ int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p,
   attr[1].val.clusterDim.x = p.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.split > 1 ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, few_rows_kernel<OP>, mw, mx, p) != cudaSuccess) return cuda_fail();
+  if (cudaLaunchKernelEx(&cfg, few_rows_kernel<OP, WIDE>, mw, mx, p) != cudaSuccess) return cuda_fail();
   return cuda_check_launch();
 }
 

@@ -61,6 +61,8 @@ static int launch_grad(const void* dh, const void* pre, void* dpre, int M, int F
   return cuda_check_launch();
 }
 
+static bool few_rows(int M) { return M <= 512; }
+
 static bool shape_ok(int M, int F, int K, int act) {
   return M >= 0 && F >= 8 && K >= 8 && F % 8 == 0 && K % 8 == 0 && act >= FP4AR_ACT_SILU && act <= FP4AR_ACT_GELU_TANH &&
          extents_ok((long long)M + 256, 2LL * F + 256) && extents_ok(K, 0);
@@ -76,11 +78,12 @@ extern "C" int fp4ar_gated_linear(const void* x, const void* wt, int M, int F, i
   if (!shape_ok(M, F, K, act)) return FP4AR_ERR_ARGUMENT;
   if (M == 0) return FP4AR_OK;
   if (!x || !wt || !h || !aligned16(x, wt, h, pre)) return FP4AR_ERR_ARGUMENT;
-  if (M <= kFewRows) {
+  if (few_rows(M)) {
     FewParams fp;
     memset(&fp, 0, sizeof(fp));
     fp.M = M; fp.N = F; fp.act = act; fp.out = (__nv_bfloat16*)h; fp.pre = (float*)pre;
-    return launch_few_rows<kGated>(wt, 2L * F, x, K, fp, (cudaStream_t)stream);
+    return M <= kNarrowRows ? launch_few_rows<kGated, false>(wt, 2L * F, x, K, fp, (cudaStream_t)stream)
+                            : launch_few_rows<kGated, true>(wt, 2L * F, x, K, fp, (cudaStream_t)stream);
   }
   Maps maps;
   memset(&maps, 0, sizeof(maps));
@@ -105,7 +108,14 @@ extern "C" int fp4ar_gated_backward(const void* dh, const void* pre, const void*
   int rc = launch_grad(dh, pre, dpre, M, F, act, stream);
   if (rc != FP4AR_OK) return rc;
   Params p;
-  if (dx) {
+  if (dx && few_rows(M)) {
+    FewParams fp;
+    memset(&fp, 0, sizeof(fp));
+    fp.M = M; fp.N = K; fp.out = (__nv_bfloat16*)dx;
+    rc = M <= kNarrowRows ? launch_few_rows<kInput, false>(wt, 2L * F, dpre, 2 * F, fp, stream)
+                          : launch_few_rows<kInput, true>(wt, 2L * F, dpre, 2 * F, fp, stream);
+    if (rc != FP4AR_OK) return rc;
+  } else if (dx) {
     Maps maps;
     memset(&maps, 0, sizeof(maps));
     memset(&p, 0, sizeof(p));
