@@ -225,7 +225,7 @@ done:
     }
     if (tid == 64) out[0] = count + scount[0] + scount[1] + scount[2] + scount[3];
   }
-  if (p.split > 1) cluster_sync_all();                   // a CTA's part is read until here
+  if (p.split > 1) cluster_sync_relaxed();               // a CTA's part is read until here
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();

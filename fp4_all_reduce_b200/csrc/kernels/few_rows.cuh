@@ -198,19 +198,19 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   // Four neighbouring outputs of a row at a time.
   const uint32_t base = smem_addr(part);
   auto sum4 = [&](int at) {
-    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int d = 0; d < p.split; d++) {
-      float4 f;
-      if (p.split > 1) {
+    if (p.split == 1) return *reinterpret_cast<const float4*>(part + at);
+    float4 f[8];                                     // all of them in flight
+#pragma unroll
+    for (int d = 0; d < 8; d++)
+      if (d < p.split) {
         uint32_t a;
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(base + at * 4), "r"(d));
-        f = cluster_ld4(a);
-      } else {
-        f = *reinterpret_cast<const float4*>(part + at);
+        f[d] = cluster_ld4(a);
       }
-      s.x += f.x; s.y += f.y; s.z += f.z; s.w += f.w;
-    }
-    return s;
+#pragma unroll
+    for (int d = 1; d < 8; d++)
+      if (d < p.split) { f[0].x += f[d].x; f[0].y += f[d].y; f[0].z += f[d].z; f[0].w += f[d].w; }
+    return f[0];
   };
   if constexpr (OP == kGated) {
     for (int i = item0 + tid; i < item1; i += 192) {
@@ -234,7 +234,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       *reinterpret_cast<uint2*>(p.out + (size_t)(first + i / 32) * p.N + n) = make_uint2(pack_bf16(s.x + low.x, s.y + low.y), pack_bf16(s.z + low.z, s.w + low.w));
     }
   }
-  if (p.split > 1) cluster_sync_all();               // a CTA's sums are read until here
+  if (p.split > 1) cluster_sync_relaxed();           // a CTA's sums are read until here
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
