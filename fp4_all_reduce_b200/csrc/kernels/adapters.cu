@@ -42,13 +42,26 @@ constexpr int kLowStage = kOpBytes + 256 * kBlockK * 2;        // x, then up to 
 __host__ __device__ constexpr int low_stages(int R) { return R <= 64 ? 4 : 3; }
 __host__ __device__ constexpr int low_smem(int R) { return low_stages(R) * kLowStage + 128 * R * 4 + 1024; }
 
+// Whether `id` is among the first `n` of sid.
+__device__ __forceinline__ bool seen_before(const int* sid, int n, int id) {
+  bool seen = false;
+#pragma unroll 8
+  for (int i = 0; i < n; i += 4) {
+    const int4 s = *reinterpret_cast<const int4*>(sid + i);
+    seen = seen | (s.x == id) | (s.y == id && i + 1 < n) | (s.z == id && i + 2 < n) | (s.w == id && i + 3 < n);
+  }
+  return seen;
+}
+__device__ __forceinline__ void rows_barrier() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }      // warps 2-5
+
 __global__ void __launch_bounds__(192, 1)
 low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ LowParams p) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kLowStages], empty[kLowStages], acc_full, acc_empty;
   __shared__ uint32_t tmem_holder;
   __shared__ volatile uint32_t abort_flag;
-  __shared__ int sid[256], list[128], scount[8], count;
+  __shared__ __align__(16) int sid[256];
+  __shared__ int list[128], scount[4], scount2[4], count;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int stages = low_stages(p.R);
   float* part = reinterpret_cast<float*>(ring + stages * kLowStage);       // [128][R]
@@ -82,8 +95,7 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   __syncthreads();
   tc_fence_after();
   if (r >= 0) {
-    first = id >= 0;
-    for (int i = 0; i < r; i++) first = first && sid[i] != id;
+    first = id >= 0 && !seen_before(sid, r, id);
     votes = __ballot_sync(0xffffffffu, first);
     if (lane == 0) scount[warp - 2] = __popc(votes);
   }
@@ -135,7 +147,24 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
     }
   } else {
-    // warps 2-5: TMEM lane quarter warp & 3 has rows 32 (warp & 3) ...
+    if ((tile & 1) == 0 && crank == 0) {
+      // the list of 256 rows for the product with W: these 128 rows' and what the other 128 add
+      sid[128 + r] = id = id_of(row0 + 128 + r);
+      rows_barrier();
+      const bool adds = id >= 0 && !seen_before(sid, 128 + r, id);
+      votes = __ballot_sync(0xffffffffu, adds);
+      if (lane == 0) scount2[warp - 2] = __popc(votes);
+      rows_barrier();
+      int* out = p.lists + (size_t)(tile >> 1) * kListStride;
+      if (r < count) out[1 + r] = list[r];
+      if (adds) {
+        int at = count + __popc(votes & ((1u << lane) - 1u));
+        for (int w = 0; w < warp - 2; w++) at += scount2[w];
+        out[1 + at] = id;
+      }
+      if (r == 0) out[0] = count + scount2[0] + scount2[1] + scount2[2] + scount2[3];
+    }
+    // TMEM lane quarter warp & 3 has rows 32 (warp & 3) ...
     const int q = warp & 3, row = q * 32 + lane;
     const int mine = sid[row];
     for (int ps = 0; ps < passes; ps++) {
@@ -203,27 +232,6 @@ done:
     uint32_t* line = reinterpret_cast<uint32_t*>(p.v + (size_t)(row0 + rr) * (2 * padded) + n / kChunk * 64 + n % kChunk);
     line[0] = hi;
     line[kChunk / 2] = pack_bf16(fabsf(l0) <= 3.4e38f ? l0 : 0.0f, fabsf(l1) <= 3.4e38f ? l1 : 0.0f);
-  }
-  if ((tile & 1) == 0 && crank == 0) {
-    // the list of 256 rows for the product with W: these 128 rows' and what the other 128 add
-    __syncthreads();
-    if (r >= 0) sid[128 + r] = id = id_of(row0 + 128 + r);
-    __syncthreads();
-    if (r >= 0) {
-      first = id >= 0;
-      for (int i = 0; i < 128 + r; i++) first = first && sid[i] != id;
-      votes = __ballot_sync(0xffffffffu, first);
-      if (lane == 0) scount[warp - 2] = __popc(votes);
-    }
-    __syncthreads();
-    int* out = p.lists + (size_t)(tile >> 1) * kListStride;
-    for (int i = tid; i < count; i += 192) out[1 + i] = list[i];
-    if (first) {
-      int at = count + __popc(votes & ((1u << lane) - 1u));
-      for (int w = 0; w < warp - 2; w++) at += scount[w];
-      out[1 + at] = id;
-    }
-    if (tid == 64) out[0] = count + scount[0] + scount[1] + scount[2] + scount[3];
   }
   if (p.split > 1) cluster_sync_relaxed();               // a CTA's part is read until here
   if (warp == 1) {

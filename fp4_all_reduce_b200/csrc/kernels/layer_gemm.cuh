@@ -44,7 +44,7 @@ constexpr int kOpBytes = kRowsCta * kBlockK * 2;               // 16 KB of A, 16
 constexpr int kStage = 2 * kOpBytes;
 constexpr int kSlab = 32 * 64 * 2;                             // 32 rows x 64 BF16 columns, one warp's store
 constexpr int kSlabs = 8 * kSlab;                              // one per epilogue warp
-constexpr int kSmemBytes = kStages * kStage + kSlabs + 512 + 1024;
+constexpr int kSmemBytes = kStages * kStage + kSlabs + 768 + 1024;
 constexpr int kListStride = 260;                               // per 256-row tile: count, then up to 256 adapters (16-byte pitch)
 constexpr int kVerdicts = 16;                                  // a granted stage is six segments ahead of the MMAs at most, these two of the epilogue
 constexpr int kChunk = 32;                                     // ranks per block of low-rank factors
@@ -182,6 +182,10 @@ struct Walk {
 // tile takes (they come from L2, under the main loop) and write zeros for A and B where one value is not finite; the
 // epilogue then adds such adapters to their own rows by plain dot products.
 constexpr int kLowThreads = 64;
+// 16 bytes into shared memory without a register in between, or zeros
+__device__ __forceinline__ void copy_or_zero(void* smem_dst, const void* gmem_src, bool copy) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(smem_dst)), "l"(gmem_src), "r"(copy ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ void low_rank_barrier() { asm volatile("barrier.cta.sync 1, 64;" ::: "memory"); }
 // ... and whether every one of the two warps' threads says yes
 __device__ __forceinline__ bool low_rank_all(bool yes) {
@@ -240,6 +244,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(granted + kStages);
   volatile uint32_t* abort_flag = tmem_holder + 1;
   volatile uint32_t* unsafe_tile = tmem_holder + 2;            // kAdapt, [kVerdicts]: 1 + the segment of which an adapter is left to the epilogue
+  uint8_t* skipped = reinterpret_cast<uint8_t*>(tmem_holder + 2 + kVerdicts);      // kAdapt, [256]: this tile's adapters that are left to the epilogue
   uint32_t issued = 0;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -375,6 +380,11 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       const int m0 = tm * 256 + (int)crank * 128, n0 = tn * 256 + (int)crank * 128;
       const int* list = p.lists + (size_t)tm * kListStride;
       const int count = list[0];
+      // which adapters of the list are left to the epilogue, before any stage is granted
+      for (int j = 0; j < count; j++) {
+        const bool all = low_rank_all(low_rank_finite(p, list[1 + j], tn * 256, lt, kLowThreads));
+        if (lt == 0) skipped[j] = !all;
+      }
       // this thread's 16 pieces of 16 bytes of a block: piece lt & 7 of rows lt / 8, + 8, ...
       int ids[16];
 #pragma unroll
@@ -382,38 +392,43 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         const int row = m0 + (lt >> 3) + 8 * i;
         ids[i] = row < p.M ? p.ids[row] : -1;
       }
-      for (int j = 0; j < count; j++) {
-        const int adapter = list[1 + j];
-        const bool all = low_rank_all(low_rank_finite(p, adapter, tn * 256, lt, kLowThreads));
-        for (int c = 0; c < chunks; c++, next++) {
-          uint4 w[16];
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int row = m0 + (lt >> 3) + 8 * i;
-            w[i] = all && ids[i] == adapter ? __ldcg(reinterpret_cast<const uint4*>(p.v + ((size_t)row * chunks + c) * 64) + (lt & 7)) : make_uint4(0, 0, 0, 0);
-          }
-          const int s = next % kStages;
+      low_rank_barrier();
+      // One block is copied into its stage while the one before it lands and is handed over.
+      const int blocks = count * chunks;
+      for (int k = 0; k <= blocks; k++) {
+        if (k < blocks) {
+          const int adapter = list[1 + k / chunks], c = k % chunks, s = (next + k) % kStages;
           if (!low_rank_all(gemm_wait(granted + s, seen >> s & 1u, gw, 1))) goto done;      // all of them or none
           seen ^= 1u << s;
-          if (!all && lt == 0) unsafe_tile[tile_i % kVerdicts] = tile_i + 1u;      // before the arrival that the MMAs wait for
+          const bool good = !skipped[k / chunks];
           uint8_t *sa = ring + s * kStage, *sb = sa + kOpBytes;
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             const int r = (lt >> 3) + 8 * i;
-            sts16(sa + r * 128 + (((lt & 7) ^ (r & 7)) << 4), w[i]);
+            const bool copy = good && ids[i] == adapter;
+            copy_or_zero(sa + r * 128 + (((lt & 7) ^ (r & 7)) << 4), copy ? p.v + ((size_t)(m0 + r) * chunks + c) * 64 + (lt & 7) * 8 : p.v, copy);
           }
-          if (!all)
+          if (good) {
+            if (lt == 0) tma_load_2d_pair(sb, &maps.low, c * kChunk, adapter * p.N + n0, cluster_addr(full + s, 0u));
+          } else {
+            if (lt == 0) unsafe_tile[tile_i % kVerdicts] = tile_i + 1u;      // before the arrival that the MMAs wait for
             for (int i = lt; i < kOpBytes / 16; i += kLowThreads) sts16(sb + 16 * i, make_uint4(0, 0, 0, 0));
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (k > 0) {
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
           fence_smem_to_async();
           low_rank_barrier();
           if (lt == 0) {
-            const uint32_t lead_full = cluster_addr(full + s, 0u);
-            if (leads) mbar_arrive_expect(full + s, all ? 2 * kOpBytes : 0);
-            else mbar_arrive_cluster(lead_full);
-            if (all) tma_load_2d_pair(sb, &maps.low, c * kChunk, adapter * p.N + n0, lead_full);
+            const int s = (next + k - 1) % kStages;
+            if (leads) mbar_arrive_expect(full + s, skipped[(k - 1) / chunks] ? 0 : 2 * kOpBytes);
+            else mbar_arrive_cluster(cluster_addr(full + s, 0u));
           }
         }
       }
+      next += (uint32_t)blocks;
+      low_rank_barrier();                       // `skipped` is read until here
     }
   } else {
     // ------------------------------------------------------------ epilogue
