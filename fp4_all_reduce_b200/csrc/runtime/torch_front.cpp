@@ -302,8 +302,7 @@ std::tuple<Tensor, Tensor> op_gated_backward(const Tensor& dh, const Tensor& pre
   return {std::move(dx), std::move(dw)};
 }
 
-// Records h for autograd.  (As a Python function the forward and backward pass cost 25 us more of host time than the launches, and the
-// backward pass took the interpreter's lock.)
+// Records h for autograd: 12 us of host time for both passes beside the autograd engine's own (as a Python function 30).
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& wt, int64_t act) {
     auto r = op_gated_linear(x, wt, act, true, Tensor());
@@ -325,7 +324,18 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     return out;
   }
 };
-Tensor op_gated_linear_recorded(const Tensor& x, const Tensor& wt, int64_t act) { return GatedLinear::apply(x, wt, act); }
+bool recording(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+// h, recorded where autograd records
+Tensor op_gated_linear_auto(const Tensor& x, const Tensor& wt, int64_t act, Tensor out) {
+  if (!recording({&x, &wt})) return std::get<0>(op_gated_linear(x, wt, act, false, std::move(out)));
+  TORCH_CHECK_VALUE(!out.defined(), "out cannot be given where a gradient is recorded");
+  return GatedLinear::apply(x, wt, act);
+}
 
 Tensor op_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, const Tensor& a, const Tensor& b, const Tensor& scales, Tensor out) {
   TORCH_CHECK_VALUE(x.dim() == 2, "x must have shape [rows, K], got ", shape_text(x));
@@ -519,24 +529,24 @@ PyObject* wrap2_or_none(std::tuple<Tensor, Tensor> r) {
   PyTuple_SET_ITEM(t.get(), 1, wrap_or_none(std::move(std::get<1>(r))));
   return t.release();
 }
-// (x, wt, activation, want_pre, out or None): (h, pre or None)
-PyObject* py_gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// (x, wt, activation, out or None): (h, pre)
+PyObject* py_gated_linear_pre(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arity(n, 5);
+  arity(n, 4);
   const Tensor &x = tensor_arg(a[0], "x"), &wt = tensor_arg(a[1], "wt");
   const int64_t act = int_arg(a[2]);
-  const bool pre = bool_arg(a[3]);
-  Tensor out = a[4] == Py_None ? Tensor() : tensor_arg(a[4], "out");
-  return wrap2_or_none([&] { NoGil g; return op_gated_linear(x, wt, act, pre, std::move(out)); }());
+  Tensor out = a[3] == Py_None ? Tensor() : tensor_arg(a[3], "out");
+  return wrap2_or_none([&] { NoGil g; return op_gated_linear(x, wt, act, true, std::move(out)); }());
   END_HANDLE_TH_ERRORS
 }
-// (x, wt, activation): h, recorded for autograd
-PyObject* py_gated_linear_recorded(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// (x, wt, activation, out or None): h, recorded where autograd records
+PyObject* py_gated_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  arity(n, 3);
+  arity(n, 4);
   const Tensor &x = tensor_arg(a[0], "x"), &wt = tensor_arg(a[1], "wt");
   const int64_t act = int_arg(a[2]);
-  return THPVariable_Wrap([&] { NoGil g; return op_gated_linear_recorded(x, wt, act); }());
+  Tensor out = a[3] == Py_None ? Tensor() : tensor_arg(a[3], "out");
+  return THPVariable_Wrap([&] { NoGil g; return op_gated_linear_auto(x, wt, act, std::move(out)); }());
   END_HANDLE_TH_ERRORS
 }
 // (dh, pre, x, wt, activation, need_dx, need_dw): (dx or None, dwt or None)
@@ -557,6 +567,8 @@ PyObject* py_linear_adapters(PyObject*, PyObject* const* p, Py_ssize_t n) {
                &b = tensor_arg(p[4], "b");
   const Tensor scales = p[5] == Py_None ? Tensor() : tensor_arg(p[5], "scales");
   Tensor out = p[6] == Py_None ? Tensor() : tensor_arg(p[6], "out");
+  if (recording({&x, &wt, &a, &b, &scales}))
+    throw std::runtime_error("linear_adapters has no backward pass: call it under torch.no_grad() or on detached tensors");
   return THPVariable_Wrap([&] { NoGil g; return op_linear_adapters(x, wt, ids, a, b, scales, std::move(out)); }());
   END_HANDLE_TH_ERRORS
 }
@@ -724,7 +736,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FP4AR_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FP4AR_METHOD(bind), FP4AR_METHOD(encode), FP4AR_METHOD(encode_static), FP4AR_METHOD(decode_sum),
-                         FP4AR_METHOD(reduce_reencode), FP4AR_METHOD(add_rmsnorm), FP4AR_METHOD(gemm), FP4AR_METHOD(gated_linear), FP4AR_METHOD(gated_linear_recorded), FP4AR_METHOD(gated_backward),
+                         FP4AR_METHOD(reduce_reencode), FP4AR_METHOD(add_rmsnorm), FP4AR_METHOD(gemm), FP4AR_METHOD(gated_linear), FP4AR_METHOD(gated_linear_pre), FP4AR_METHOD(gated_backward),
                          FP4AR_METHOD(linear_adapters), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fp4ar_front", nullptr, -1, methods};
 

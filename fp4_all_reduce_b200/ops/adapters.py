@@ -23,6 +23,4 @@ from .. import _native as N
 def linear_adapters(x: torch.Tensor, wt: torch.Tensor, ids: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
                     scales: Optional[torch.Tensor] = None, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x @ wt.T plus every row's own adapter, BF16 [M, N] (into `out` when given)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, wt, a, b, scales)):
-        raise RuntimeError("linear_adapters has no backward pass: call it under torch.no_grad() or on detached tensors")
     return N.front().linear_adapters(x, wt, ids, a, b, scales, out)

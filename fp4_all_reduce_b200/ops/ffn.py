@@ -27,17 +27,13 @@ ACTIVATIONS = {"silu": N.ACT_SILU, "gelu": N.ACT_GELU, "gelu_tanh": N.ACT_GELU_T
 def gated_linear(x: torch.Tensor, wt: torch.Tensor, activation: int = N.ACT_SILU, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x @ wt[:F].T) * (x @ wt[F:].T).  Where autograd records, the projections are kept for the backward pass and `out`
     cannot be given."""
-    if torch.is_grad_enabled() and (x.requires_grad or wt.requires_grad):
-        if out is not None:
-            raise ValueError("out cannot be given where a gradient is recorded")
-        return N.front().gated_linear_recorded(x, wt, activation)
-    return N.front().gated_linear(x, wt, activation, False, out)[0]
+    return N.front().gated_linear(x, wt, activation, out)
 
 
 def gated_linear_forward(x: torch.Tensor, wt: torch.Tensor, activation: int = N.ACT_SILU, *,
                          out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(h, pre): pre [M, 2 F] holds the gate and the up projections in FP32; h is the same as without it.  Records no gradient."""
-    return N.front().gated_linear(x, wt, activation, True, out)
+    return N.front().gated_linear_pre(x, wt, activation, out)
 
 
 def gated_linear_backward(dh: torch.Tensor, pre: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, activation: int = N.ACT_SILU, *,

@@ -17,8 +17,8 @@ def act(g, kind):
     if kind == 0:
         return g * torch.sigmoid(g)
     if kind == 1:
-        return g * torch.special.ndtr(g)
-    return 0.5 * g * (1 + torch.tanh(math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)))
+        return 0.5 * g * torch.special.erfc(-g / math.sqrt(2))      # (ndtr cancels for negative g: 0 instead of 1.1e-19 at -9)
+    return g * torch.sigmoid(math.sqrt(8 / math.pi) * (g + 0.044715 * g ** 3))      # (1 + tanh z) / 2 without its cancellation
 
 
 def act_grad(g, kind):

@@ -74,3 +74,110 @@ def test_a_broken_adapter_stays_with_its_rows(M, where):
         keep = [c for c in range(264) if c not in (5, 6)]
         want, bound = R.adapters(x, wt, ids, a, b, sc)
         assert bool(((y.double() - want).abs() <= bound)[mine][:, keep].all())
+
+
+def test_no_rows_out_and_the_custom_op():
+    x, wt, ids, a, b, sc = _data(20, 72, 40, 3, 8, 4)
+    assert AD.linear_adapters(x[:0], wt, ids[:0], a, b, sc).shape == (0, 40)
+    y = _check((x, wt, ids, a, b, sc))
+    room = torch.full((22, 40), 7.0, device="cuda", dtype=torch.bfloat16)
+    out = AD.linear_adapters(x, wt, ids, a, b, sc, out=room[:20])
+    assert out.data_ptr() == room.data_ptr() and torch.equal(out, y) and bool((room[20:] == 7).all())
+    assert torch.equal(torch.ops.fp4ar.linear_adapters(x, wt, ids, a, b, sc), y)
+    fn = torch.compile(lambda *t: torch.ops.fp4ar.linear_adapters(*t), fullgraph=True, backend="eager")
+    assert torch.equal(fn(x, wt, ids, a, b, sc), y)
+
+
+@pytest.mark.parametrize("M", [4, 300])
+def test_every_rank_and_every_adapter_counts(M):
+    """One nonzero rank at a time, in the last adapter too: nothing of B or A is skipped or taken twice."""
+    K, Nn, n = 64, 264, 5
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(M, K, generator=g, device="cuda").to(torch.bfloat16)
+    wt = torch.zeros(Nn, K, device="cuda", dtype=torch.bfloat16)
+    ids = (torch.arange(M, device="cuda") % n).to(torch.int32)
+    for r in (8, 40, 128):
+        for at in range(0, r, 7):
+            a = torch.zeros(n, r, K, device="cuda", dtype=torch.bfloat16)
+            b = torch.zeros(n, Nn, r, device="cuda", dtype=torch.bfloat16)
+            a[:, at, 0] = torch.arange(1, n + 1, device="cuda").to(torch.bfloat16)
+            b[:, :, at] = 1.0
+            y = AD.linear_adapters(x, wt, ids, a, b)
+            want = (x[:, 0].double() * (ids + 1)).unsqueeze(1).expand(M, Nn)
+            assert bool(((y.double() - want).abs() <= (R.BF16 + 2.0 ** -16) * want.abs()).all()), (r, at)
+
+
+@pytest.mark.parametrize("M", [5, 300])
+def test_offsets_beyond_32_bits(M):
+    """b has 2.6e9 elements; the last adapters and the last columns are looked at."""
+    n, Nn, r, K = 160, 131072, 128, 8
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(M, K, generator=g, device="cuda").to(torch.bfloat16)
+    wt = torch.randn(Nn, K, generator=g, device="cuda").to(torch.bfloat16)
+    a = torch.randn(n, r, K, generator=g, device="cuda").to(torch.bfloat16)
+    b = torch.empty(n, Nn, r, device="cuda", dtype=torch.bfloat16)
+    b[n - 2:].normal_(generator=g)
+    b[:n - 2] = float("nan")                                         # nobody's
+    ids = (n - 1 - torch.arange(M, device="cuda") % 2).to(torch.int32)
+    y = AD.linear_adapters(x, wt, ids, a, b)
+    cols = torch.tensor([0, 1, 255, 256, 65535, 65536, Nn - 257, Nn - 1], device="cuda")
+    want, bound = R.adapters(x, wt[cols], ids - (n - 2), a[n - 2:], b[n - 2:][:, cols], None)
+    assert bool(((y[:, cols].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("M", [6, 500, 3000])
+def test_captured_and_replayed_beside_eager_calls(M):
+    x, wt, ids, a, b, sc = _data(M, 1024, 2048, 9, 24, 5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        AD.linear_adapters(x, wt, ids, a, b, sc)
+    side.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        y = AD.linear_adapters(x, wt, ids, a, b, sc)
+    torch.cuda.synchronize()
+    for seed in (6, 7, 8):
+        x2, _, ids2, a2, b2, sc2 = _data(M, 1024, 2048, 9, 24, seed)
+        x.copy_(x2), ids.copy_(ids2), a.copy_(a2), b.copy_(b2), sc.copy_(sc2)
+        torch.cuda.synchronize()
+        graph.replay()
+        y2 = AD.linear_adapters(x2, wt, ids2, a2, b2, sc2)
+        torch.cuda.synchronize()
+        assert torch.equal(y, y2)
+    assert G.gemm_status().code == 0
+
+
+def test_many_calls_in_a_row_give_the_same_bits():
+    """Back-to-back launches overlap at their ends; every one sees its own V, lists and flags."""
+    sets = [_data(m, 520, 1032, 20, 16, 30 + i) for i, m in enumerate((1, 64, 128, 129, 600, 1500))]
+    want = [AD.linear_adapters(*s) for s in sets]
+    torch.cuda.synchronize()
+    got = [(i % 6, AD.linear_adapters(*sets[i % 6])) for i in range(60)]
+    assert all(torch.equal(y, want[i]) for i, y in got)
+    assert G.gemm_status().code == 0
+
+
+def test_refusals():
+    x, wt, ids, a, b, sc = _data(4, 16, 24, 3, 8)
+    ok = dict(x=x, wt=wt, ids=ids, a=a, b=b, scales=sc)
+    for name, bad, why in (("x", x.half(), "x must be torch.bfloat16"), ("x", x[:, :8], "wt must have shape"), ("x", x.t().contiguous().t(), "contiguous"),
+                           ("wt", wt[:20], "multiples of 8"), ("wt", wt.cpu(), "CUDA"), ("ids", ids.long(), "ids must be torch.int32"),
+                           ("ids", ids[:3], "ids must have shape"), ("ids", ids.cpu(), "CUDA"), ("ids", ids.repeat(2)[::2], "contiguous"),
+                           ("a", a[:, :, :8], "a must have shape"), ("a", a[:, :4], "multiple of 8"), ("a", a[:0], "at least one"),
+                           ("a", a.float(), "a must be"), ("b", b[:2], "b must have shape"), ("b", b[:, :, :4], "b must have shape"),
+                           ("b", b.transpose(1, 2).contiguous().transpose(1, 2), "b must be contiguous"), ("scales", sc.half(), "scales must be torch.float32"),
+                           ("scales", sc[:2], "scales must have shape"), ("scales", sc.cpu(), "CUDA")):
+        with pytest.raises(ValueError, match=why):
+            AD.linear_adapters(**{**ok, name: bad})
+    with pytest.raises(ValueError, match="up to 128"):
+        AD.linear_adapters(x, wt, ids, torch.zeros(3, 136, 16, device="cuda", dtype=torch.bfloat16),
+                           torch.zeros(3, 24, 136, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="out must have shape"):
+        AD.linear_adapters(**ok, out=x)
+    with pytest.raises(ValueError, match="overlap b"):
+        AD.linear_adapters(**ok, out=b.view(-1)[:96].view(4, 24))
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        AD.linear_adapters(**{**ok, "a": a.clone().requires_grad_()})
+    with torch.no_grad():
+        AD.linear_adapters(**{**ok, "a": a.clone().requires_grad_()})
