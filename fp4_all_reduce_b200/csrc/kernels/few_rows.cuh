@@ -35,6 +35,9 @@ __device__ __forceinline__ float4 cluster_ld4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(addr));
   return f;
 }
+__device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ float act_any(int act, float g) {
   return act == FP4AR_ACT_SILU ? act_value<FP4AR_ACT_SILU>(g) : act == FP4AR_ACT_GELU ? act_value<FP4AR_ACT_GELU>(g) : act_value<FP4AR_ACT_GELU_TANH>(g);
 }
@@ -71,11 +74,17 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   GemmWait gw{&abort_flag, p.status, p.timeout_ns};
   // kAdapt: the launch before this one lets it start only after its own wait, so everything before that one is complete here; what
   // that one itself writes (V) is waited for where it is read.
+  // The first weights are asked into L2 before that wait: whoever writes them before it writes them there.
+  const int kb0 = p.kblocks * crank / p.split, kb1 = p.kblocks * (crank + 1) / p.split;
+  const int row0 = OP == kGated ? tile * 64 : tile * 128, row1 = OP == kGated ? p.N + row0 : row0 + 64;
+  if (warp == 0 && lane < p.stages && kb0 + lane < kb1) {
+    const int k = (kb0 + lane) * kBlockK;
+    prefetch_tile(&map_w, OP == kInput ? row0 : k, OP == kInput ? k : row0);
+    prefetch_tile(&map_w, OP == kInput ? row1 : k, OP == kInput ? k : row1);
+  }
   if (OP != kAdapt) pdl_wait_prior_grids();
   pdl_release_dependents();
 
-  const int kb0 = p.kblocks * crank / p.split, kb1 = p.kblocks * (crank + 1) / p.split;
-  const int row0 = OP == kGated ? tile * 64 : tile * 128, row1 = OP == kGated ? p.N + row0 : row0 + 64;
   // this CTA's share of the outputs, in groups of four
   const int items = rows * (OP == kGated ? 16 : 32), item0 = items * crank / p.split, item1 = items * (crank + 1) / p.split;
   float4* lows = reinterpret_cast<float4*>(ring + p.low_offset);
