@@ -15,6 +15,7 @@ namespace fp4ar {
 namespace layer {
 
 constexpr int kNarrowRows = 128, kFewStagesMax = 8;
+template <int OP> constexpr int kFewThreads = OP == kAdapt ? 320 : 192;      // kAdapt: four more warps for the low-rank parts
 
 struct FewParams {
   int M, N, kblocks, split, stages, tokens, groups;      // tokens: rows of a group, a multiple of 16; N: columns of the output
@@ -43,7 +44,7 @@ __device__ __forceinline__ float act_any(int act, float g) {
 }
 
 template <int OP, bool WIDE>
-__global__ void __launch_bounds__(192, WIDE ? 1 : 2)
+__global__ void __launch_bounds__(kFewThreads<OP>, WIDE ? 1 : 2)
 few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ FewParams p) {
   static_assert(OP == kGated || OP == kInput || (OP == kAdapt && !WIDE), "products with W");
   extern __shared__ uint8_t smem_raw[];
@@ -137,11 +138,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       };
       const int m0 = item0 / 32 + warp - 2, m1 = (item1 + 31) / 32;
       int from, to;
-      for (int m = m0; m < m1; m += 4)
+      for (int m = m0; m < m1; m += 8)
         if (const uint4* b = share_of(m, from, to))
           for (int o = from * pieces + lane * 8; o < to * pieces; o += 32 * 8) asm volatile("prefetch.global.L2 [%0];" ::"l"(b + o));
       pdl_wait_prior_grids();
-      for (int m = m0; m < m1; m += 4) {
+      for (int m = m0; m < m1; m += 8) {
         const uint4* b = share_of(m, from, to);
         float* low = reinterpret_cast<float*>(lows) + m * 128 - 4 * item0;
         if (!b) {
@@ -183,7 +184,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       }
     }
     const int q = warp & 3;
-    if (__all_sync(0xffffffffu, gemm_wait(&acc_full, 0u, gw, 4)) && !__any_sync(0xffffffffu, abort_flag != 0u)) {
+    if (warp < 6 && __all_sync(0xffffffffu, gemm_wait(&acc_full, 0u, gw, 4)) && !__any_sync(0xffffffffu, abort_flag != 0u)) {
       tc_fence_after();
       for (int c = 0; c < p.tokens; c += 16) {
         float v[16];
@@ -222,7 +223,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     return f[0];
   };
   if constexpr (OP == kGated) {
-    for (int i = item0 + tid; i < item1; i += 192) {
+    for (int i = item0 + tid; i < item1; i += kFewThreads<OP>) {
       const int c = i % 16 * 4, f = row0 + c;
       if (f >= p.N) continue;
       const float4 g = sum4(i / 16 * 128 + c), u = sum4(i / 16 * 128 + 64 + c);
@@ -236,7 +237,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       *reinterpret_cast<uint2*>(p.out + (size_t)m * p.N + f) = h;
     }
   } else {
-    for (int i = item0 + tid; i < item1; i += 192) {
+    for (int i = item0 + tid; i < item1; i += kFewThreads<OP>) {
       const int c = i % 32 * 4, n = row0 + c;
       if (n >= p.N) continue;
       const float4 s = sum4(i / 32 * 128 + c), low = OP == kAdapt ? lows[i - item0] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -254,7 +255,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 // Stands in for few_rows_kernel where the runtime is asked how many clusters fit: for a kernel that allocates TMEM it answers with one CTA
 // an SM whatever the kernel takes (two were seen to run side by side).
 template <int OP, bool WIDE>
-__global__ void __launch_bounds__(192, WIDE ? 1 : 2) few_rows_room_kernel() {}
+__global__ void __launch_bounds__(kFewThreads<OP>, WIDE ? 1 : 2) few_rows_room_kernel() {}
 
 // `w` has `rows` rows: 2 N of K columns (kGated), N (kAdapt), K rows of N columns (kInput).
 template <int OP, bool WIDE>
@@ -273,7 +274,7 @@ int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p,
       cudaLaunchConfig_t cfg;
       memset(&cfg, 0, sizeof(cfg));
       cfg.gridDim = dim3(64 * c);
-      cfg.blockDim = dim3(192);
+      cfg.blockDim = dim3(kFewThreads<OP>);
       cfg.dynamicSmemBytes = kBudget + 256;          // and the barriers
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -307,7 +308,7 @@ int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p,
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(tiles * p.split);
-  cfg.blockDim = dim3(192);
+  cfg.blockDim = dim3(kFewThreads<OP>);
   p.low_offset = p.stages * stage > sums ? p.stages * stage : sums;
   cfg.dynamicSmemBytes = p.low_offset + lows + 1024;
   cfg.stream = stream;
