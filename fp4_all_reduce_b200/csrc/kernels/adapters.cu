@@ -323,6 +323,13 @@ __global__ void __launch_bounds__(256, 3) few_low_rank_kernel(const __nv_bfloat1
   }
 }
 
+// Which of the two products takes a call.  A tile of 256 rows pays 1.2 us and more for every adapter in it, the few-row kernel nothing,
+// but it reads W once for every 128 rows and B once for every row.  N = 6144, K = 2048, rank 16, us, few-row kernel / tiles: 128 rows
+// of 4 adapters 19 / 28; 200 rows of 4: 23 / 27, of 16: 24 / 45, of 64: 24 / 128; 512 rows of 8: 35 / 28, of 64: 37 / 130.  Rank 64,
+// K = 8192: 256 rows of 8: 97 / 72, of 64: 103 / 427.  How many adapters a tile has is known on the device alone, so the pool's
+// size stands in for it.
+static bool few_rows(int M, int adapters) { return M <= kNarrowRows || (M <= 512 && 16LL * adapters >= M); }
+
 }  // namespace layer
 }  // namespace fp4ar
 
@@ -349,7 +356,7 @@ extern "C" int fp4ar_linear_adapters(const void* x, const void* wt, const int* i
     return FP4AR_ERR_ARGUMENT;
   const cudaStream_t stream = (cudaStream_t)stream_;
   const Workspace ws(workspace, M, R);
-  if (M <= kNarrowRows) {
+  if (few_rows(M, adapters)) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(M, R / 8);

@@ -133,7 +133,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       auto share_of = [&](int m, int& from, int& to) -> const uint4* {      // B_a from row `row0` on, rows [from, to) of the tile
         from = max(4 * item0 - m * 128, 0);
         to = min(min(4 * item1 - m * 128, 128), p.N - row0);
-        const int id = p.ids[m];
+        const int id = p.ids[first + m];
         return id >= 0 && id < p.adapters ? reinterpret_cast<const uint4*>(p.b + ((size_t)id * p.N + row0) * p.R) : nullptr;
       };
       const int m0 = item0 / 32 + warp - 2, m1 = (item1 + 31) / 32;
@@ -151,7 +151,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         }
         float v[8];
         const int piece = min(sub, pieces - 1);          // (lanes beyond the last piece read it too and add nothing)
-        const uint4* at = reinterpret_cast<const uint4*>(p.v + (size_t)m * line + piece / 4 * 64 + piece % 4 * 8);
+        const uint4* at = reinterpret_cast<const uint4*>(p.v + (size_t)(first + m) * line + piece / 4 * 64 + piece % 4 * 8);
         const uint4 hi = __ldcg(at), lo = __ldcg(at + kChunk / 8);
         const uint32_t h4[4] = {hi.x, hi.y, hi.z, hi.w}, l4[4] = {lo.x, lo.y, lo.z, lo.w};
 #pragma unroll
@@ -290,24 +290,32 @@ int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p,
   p.status = gemm_status_word();
   if (!p.status) return cuda_fail();
   p.timeout_ns = kWaitLimitNs;
-  p.groups = WIDE ? (p.M + 255) / 256 : 1;
-  p.tokens = ((p.M + p.groups - 1) / p.groups + 15) / 16 * 16;
   p.kblocks = (K + 63) / 64;
+  const int most = WIDE ? 256 : kNarrowRows, per_tile = OP == kGated ? 64 : 128;
+  long tiles;
+  int lows, sums;                                    // bytes for the low-rank parts and for the sums (which take the ring's place)
+  for (int g = (p.M + most - 1) / most;; g++) {
+    p.tokens = ((p.M + g - 1) / g + 15) / 16 * 16;
+    p.groups = (p.M + p.tokens - 1) / p.tokens;      // (rounding up may leave nothing for the last one)
+    tiles = ((long)p.N + per_tile - 1) / per_tile * p.groups;
+    // the widest split whose clusters are all resident at once (of six CTAs 45 fit, not 49: a cluster stays within a part of the GPU)
+    p.split = 1;
+    for (int c = 2; c <= 8 && 2 * c <= p.kblocks; c++)
+      if (tiles <= clusters[dev][c].load(std::memory_order_acquire)) p.split = c;
+    sums = p.tokens * 512;
+    lows = OP == kAdapt ? ((p.tokens * 32 + p.split - 1) / p.split + 1) * 16 : 0;
+    if (sums + lows <= kBudget - 1024) break;        // 128 rows of one CTA with their low-rank parts are too many
+  }
+  if (tiles * p.split > 0x7fffffffL) return FP4AR_ERR_ARGUMENT;
   CUtensorMap mw, mx;
   if (!map_2d(&mw, w, rows, OP == kInput ? p.N : K, 64) || !map_2d(&mx, x, p.M, K, p.tokens)) return FP4AR_ERR_UNSUPPORTED;
-  const int per_tile = OP == kGated ? 64 : 128, tiles = (p.N + per_tile - 1) / per_tile * p.groups;
-  // the widest split whose clusters are all resident at once (of six CTAs 45 fit, not 49: a cluster stays within a part of the GPU)
-  p.split = 1;
-  for (int c = 2; c <= 8 && 2 * c <= p.kblocks; c++)
-    if (tiles <= clusters[dev][c].load(std::memory_order_acquire)) p.split = c;
-  const int stage = kOpBytes + p.tokens * 128, blocks = (p.kblocks + p.split - 1) / p.split, sums = p.tokens * 512;
-  const int lows = OP == kAdapt ? ((p.M * 32 + p.split - 1) / p.split + 1) * 16 : 0;
+  const int stage = kOpBytes + p.tokens * 128, blocks = (p.kblocks + p.split - 1) / p.split;
   p.stages = (kBudget - 1024 - lows) / stage;
   if (p.stages > kFewStagesMax) p.stages = kFewStagesMax;
   if (p.stages > blocks) p.stages = blocks;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(tiles * p.split);
+  cfg.gridDim = dim3((unsigned)(tiles * p.split));
   cfg.blockDim = dim3(kFewThreads<OP>);
   p.low_offset = p.stages * stage > sums ? p.stages * stage : sums;
   cfg.dynamicSmemBytes = p.low_offset + lows + 1024;

@@ -181,7 +181,7 @@ struct Walk {
 // 0 x infinity would leak one request's broken adapter into the rows of others: those warps look through the 256 rows of B_a that a
 // tile takes (they come from L2, under the main loop) and write zeros for A and B where one value is not finite; the
 // epilogue then adds such adapters to their own rows by plain dot products.
-constexpr int kLowThreads = 64;
+constexpr int kLowThreads = 64, kLowAhead = 3;      // (fewer than the ring's stages: a grant needs the blocks six before it handed over)
 // 16 bytes into shared memory without a register in between, or zeros
 __device__ __forceinline__ void copy_or_zero(void* smem_dst, const void* gmem_src, bool copy) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(smem_dst)), "l"(gmem_src), "r"(copy ? 16 : 0) : "memory");
@@ -200,21 +200,22 @@ __device__ __forceinline__ bool low_rank_all(bool yes) {
 
 // Not zero where one of two BF16 values is infinite or NaN (all eight exponent bits set).
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
-// Rows n0 .. n0 + 255 (below N) of B of one adapter: are all values finite?  By `lanes` lanes, each with its own answer.
-__device__ __forceinline__ bool low_rank_finite(const Params& p, int adapter, int n0, int lane, int lanes) {
+// Rows n0 .. n0 + 255 (below N) of B of one adapter: are all values finite?  By a warp (every lane has the answer) or by one thread.
+template <int LANES>
+__device__ __forceinline__ bool low_rank_finite(const Params& p, int adapter, int n0, int lane) {
   const uint4* b = reinterpret_cast<const uint4*>(p.b + ((size_t)adapter * p.N + n0) * p.R);
   const int n = min(256, p.N - n0) * (p.R / 8);
   uint32_t bad = 0;
-  for (int i = lane; i < n; i += 16 * lanes) {               // sixteen loads in flight
+  for (int i = lane; i < n; i += 16 * LANES) {               // sixteen loads in flight
     uint4 w[16];
 #pragma unroll
-    for (int j = 0; j < 16; j++) w[j] = i + j * lanes < n ? __ldg(b + i + j * lanes) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < 16; j++) w[j] = __ldg(b + min(i + j * LANES, n - 1));
 #pragma unroll
     for (int j = 0; j < 16; j++) bad |= not_finite(w[j].x) | not_finite(w[j].y) | not_finite(w[j].z) | not_finite(w[j].w);
   }
-  return bad == 0;
+  return LANES == 1 ? bad == 0 : (bool)__all_sync(0xffffffffu, bad == 0);
 }
-static __device__ __noinline__ bool low_rank_unsafe(const Params& p, int adapter, int n0) { return !low_rank_finite(p, adapter, n0, 0, 1); }
+static __device__ __noinline__ bool low_rank_unsafe(const Params& p, int adapter, int n0) { return !low_rank_finite<1>(p, adapter, n0, 0); }
 
 static __device__ __noinline__ float low_rank_dot(const __nv_bfloat16* v, const __nv_bfloat16* b, int R) {
   float s = 0.0f;
@@ -241,7 +242,8 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* settled = acc_empty + 2;
   uint64_t* granted = settled + 1;             // kAdapt, [kStages]: the stage is free for a block of low-rank factors
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(granted + kStages);
+  uint64_t* filled = granted + kStages;        // kAdapt, [kStages], second CTA: its half of such a block is written
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(filled + kStages);
   volatile uint32_t* abort_flag = tmem_holder + 1;
   volatile uint32_t* unsafe_tile = tmem_holder + 2;            // kAdapt, [kVerdicts]: 1 + the segment of which an adapter is left to the epilogue
   uint8_t* skipped = reinterpret_cast<uint8_t*>(tmem_holder + 2 + kVerdicts);      // kAdapt, [256]: this tile's adapters that are left to the epilogue
@@ -256,7 +258,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
 
   if (threadIdx.x == 0) {
     // kAdapt: two arrivals, since both CTAs write into a stage of low-rank factors themselves
-    for (int s = 0; s < kStages; s++) { mbar_init(full + s, OP == kAdapt ? 2 : 1); mbar_init(empty + s, 1); mbar_init(granted + s, 1); }
+    for (int s = 0; s < kStages; s++) { mbar_init(full + s, OP == kAdapt ? 2 : 1); mbar_init(empty + s, 1); mbar_init(granted + s, 1); mbar_init(filled + s, 1); }
     for (int a = 0; a < 2; a++) { mbar_init(acc_full + a, 1); mbar_init(acc_empty + a, 16); }
     mbar_init(settled, 1);
     *abort_flag = 0u;
@@ -366,6 +368,23 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         }
         umma_commit_pair(acc_full + a);
       }
+    } else if (OP == kAdapt && lane == 0) {
+      // The second CTA's warp hands its blocks of low-rank factors over to the leader: an arrival that releases at cluster scope waits for
+      // all that its thread has in flight, which in the warps that copy would be the next blocks (1.6 us a block instead of 1.2).
+      uint32_t next = 0, seen = 0;
+      while (walk.next(sg)) {
+        next += (uint32_t)sg.count;
+        if (sg.kind == kProduce) continue;
+        int tm, tn;
+        tile_at(sg.tile, m_tiles, n_tiles, tm, tn);
+        const int blocks = p.lists[(size_t)tm * kListStride] * ((p.R + kChunk - 1) / kChunk);
+        for (int i = 0; i < blocks; i++, next++) {
+          const int s = next % kStages;
+          if (!gemm_wait(filled + s, seen >> s & 1u, gw, 1)) goto done;
+          seen ^= 1u << s;
+          mbar_arrive_cluster(cluster_addr(full + s, 0u));
+        }
+      }
     }
   } else if (OP == kAdapt && warp >= 10) {
     // ------------------------------------------------------------ blocks of low-rank factors
@@ -381,9 +400,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       const int* list = p.lists + (size_t)tm * kListStride;
       const int count = list[0];
       // which adapters of the list are left to the epilogue, before any stage is granted
-      for (int j = 0; j < count; j++) {
-        const bool all = low_rank_all(low_rank_finite(p, list[1 + j], tn * 256, lt, kLowThreads));
-        if (lt == 0) skipped[j] = !all;
+      for (int j = warp - 10; j < count; j += 2) {
+        const bool good = low_rank_finite<32>(p, list[1 + j], tn * 256, lane);
+        if (lane == 0) skipped[j] = !good;
       }
       // this thread's 16 pieces of 16 bytes of a block: piece lt & 7 of rows lt / 8, + 8, ...
       int ids[16];
@@ -393,9 +412,10 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         ids[i] = row < p.M ? p.ids[row] : -1;
       }
       low_rank_barrier();
-      // One block is copied into its stage while the one before it lands and is handed over.
+      // Blocks are copied into their stages while up to three before them land and are handed over.  (With one before them and the
+      // checks by both warps together a block took 1.9 us: 272 us for 128 rows of 128 adapters.)
       const int blocks = count * chunks;
-      for (int k = 0; k <= blocks; k++) {
+      for (int k = 0; k < blocks + kLowAhead; k++) {
         if (k < blocks) {
           const int adapter = list[1 + k / chunks], c = k % chunks, s = (next + k) % kStages;
           if (!low_rank_all(gemm_wait(granted + s, seen >> s & 1u, gw, 1))) goto done;      // all of them or none
@@ -416,14 +436,14 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        if (k > 0) {
-          asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (k >= kLowAhead) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kLowAhead) : "memory");
           fence_smem_to_async();
           low_rank_barrier();
           if (lt == 0) {
-            const int s = (next + k - 1) % kStages;
-            if (leads) mbar_arrive_expect(full + s, skipped[(k - 1) / chunks] ? 0 : 2 * kOpBytes);
-            else mbar_arrive_cluster(cluster_addr(full + s, 0u));
+            const int s = (next + k - kLowAhead) % kStages;
+            if (leads) mbar_arrive_expect(full + s, skipped[(k - kLowAhead) / chunks] ? 0 : 2 * kOpBytes);
+            else mbar_arrive(filled + s);
           }
         }
       }

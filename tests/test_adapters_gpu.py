@@ -4,6 +4,7 @@ import torch
 
 import layer_ref as R
 from fp4_all_reduce_b200.ops import adapters as AD
+from fp4_all_reduce_b200.ops import allreduce as A  # noqa: F401  (registers torch.ops.fp4ar)
 from fp4_all_reduce_b200.ops import gemm as G
 
 pytestmark = pytest.mark.gpu
@@ -74,6 +75,12 @@ def test_a_broken_adapter_stays_with_its_rows(M, where):
         keep = [c for c in range(264) if c not in (5, 6)]
         want, bound = R.adapters(x, wt, ids, a, b, sc)
         assert bool(((y.double() - want).abs() <= bound)[mine][:, keep].all())
+
+
+@pytest.mark.parametrize("M,K,Nn", [(128, 64, 264), (112, 72, 520), (128, 256, 40000), (256, 64, 136), (250, 2048, 6144), (225, 128, 1000), (500, 136, 264)])
+def test_many_rows_of_one_tile(M, K, Nn):
+    """Short K loops and wide outputs leave K whole: a CTA then holds the sums and the low-rank parts of all its rows."""
+    _check(_data(M, K, Nn, 40, 16, 6))
 
 
 def test_no_rows_out_and_the_custom_op():
