@@ -61,7 +61,15 @@ static int launch_grad(const void* dh, const void* pre, void* dpre, int M, int F
   return cuda_check_launch();
 }
 
-static bool few_rows(int M) { return M <= 512; }
+// Which kernel takes a product of M rows whose output has `cols` columns, `per_tile` of them to a tile of 256 rows: up to 128 rows the one
+// for few rows, and up to 1024 where the other would keep no more than a third of the units busy.  us, few-row kernel / tiles, forward:
+// K = 6144, F = 2048: 200 rows (16 tiles) 20 / 29, 333 (32 tiles) 30 / 32, 512 (32) 34 / 33; F = 8192: 200 rows (64) 51 / 44.  dx of K = 2048, F = 2056:
+// 512 rows (16 tiles) 22 / 30, 640 (24) 29 / 30, 1024 (32) 32 / 30; of K = 6144, F = 2048: 256 rows (24) 28 / 27, 333 (48) 36 / 29.
+static bool few_rows(int M, int cols, int per_tile) {
+  if (M <= kNarrowRows) return true;
+  const long tiles = (M + 255L) / 256 * ((cols + per_tile - 1L) / per_tile);
+  return M <= 1024 && 3 * tiles <= device_sm_count() / 2;
+}
 
 static bool shape_ok(int M, int F, int K, int act) {
   return M >= 0 && F >= 8 && K >= 8 && F % 8 == 0 && K % 8 == 0 && act >= FP4AR_ACT_SILU && act <= FP4AR_ACT_GELU_TANH &&
@@ -78,7 +86,7 @@ extern "C" int fp4ar_gated_linear(const void* x, const void* wt, int M, int F, i
   if (!shape_ok(M, F, K, act)) return FP4AR_ERR_ARGUMENT;
   if (M == 0) return FP4AR_OK;
   if (!x || !wt || !h || !aligned16(x, wt, h, pre)) return FP4AR_ERR_ARGUMENT;
-  if (few_rows(M)) {
+  if (few_rows(M, F, 128)) {
     FewParams fp;
     memset(&fp, 0, sizeof(fp));
     fp.M = M; fp.N = F; fp.act = act; fp.out = (__nv_bfloat16*)h; fp.pre = (float*)pre;
@@ -108,7 +116,7 @@ extern "C" int fp4ar_gated_backward(const void* dh, const void* pre, const void*
   int rc = launch_grad(dh, pre, dpre, M, F, act, stream);
   if (rc != FP4AR_OK) return rc;
   Params p;
-  if (dx && few_rows(M)) {
+  if (dx && few_rows(M, K, 256)) {
     FewParams fp;
     memset(&fp, 0, sizeof(fp));
     fp.M = M; fp.N = K; fp.out = (__nv_bfloat16*)dx;
