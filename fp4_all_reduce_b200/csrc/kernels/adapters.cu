@@ -37,10 +37,11 @@ struct LowParams {
 // epilogue keeps of each row the columns of its own adapter.  So what another adapter or row holds reaches nobody else, and the
 // time is that of reading x.  A cluster of `split` CTAs cuts K where there are few rows; their sums meet in shared memory, in the
 // order of the CTAs.
-constexpr int kLowStages = 4;
-constexpr int kLowStage = kOpBytes + 256 * kBlockK * 2;        // x, then up to 256 rows of A
-__host__ __device__ constexpr int low_stages(int R) { return R <= 64 ? 4 : 3; }
-__host__ __device__ constexpr int low_smem(int R) { return low_stages(R) * kLowStage + 128 * R * 4 + 1024; }
+// The ring's stages are as large as the adapters of the rows need (8192 x 8192, rank 64: four stages for 256 rows of A 42 us, eight for one
+// adapter 38, which is 151 MB at 4.0 TB/s, launch, lists and the exchange of the sums, about 5 us, included; 4096 x 2048, rank 16: 12 us).
+constexpr int kLowStagesMax = 10;
+__host__ __device__ constexpr int low_ring(int R) { return (R <= 64 ? 4 : 3) * (kOpBytes + 256 * kBlockK * 2); }
+__host__ __device__ constexpr int low_smem(int R) { return low_ring(R) + 128 * R * 4 + 1024; }
 
 // Whether `id` is among the first `n` of sid.
 __device__ __forceinline__ bool seen_before(const int* sid, int n, int id) {
@@ -57,18 +58,17 @@ __device__ __forceinline__ void rows_barrier() { asm volatile("barrier.cta.sync 
 __global__ void __launch_bounds__(192, 1)
 low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ LowParams p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kLowStages], empty[kLowStages], acc_full, acc_empty;
+  __shared__ uint64_t full[kLowStagesMax], empty[kLowStagesMax], acc_full, acc_empty;
   __shared__ uint32_t tmem_holder;
   __shared__ volatile uint32_t abort_flag;
   __shared__ __align__(16) int sid[256];
   __shared__ int list[128], scount[4], scount2[4], count;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int stages = low_stages(p.R);
-  float* part = reinterpret_cast<float*>(ring + stages * kLowStage);       // [128][R]
+  float* part = reinterpret_cast<float*>(ring + low_ring(p.R));            // [128][R]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tile = blockIdx.x / p.split, crank = blockIdx.x % p.split, row0 = tile * 128;
   if (tid == 0) {
-    for (int s = 0; s < stages; s++) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
+    for (int s = 0; s < kLowStagesMax; s++) { mbar_init(full + s, 1); mbar_init(empty + s, 1); }
     mbar_init(&acc_full, 1);
     mbar_init(&acc_empty, 4);
     abort_flag = 0u;
@@ -110,6 +110,7 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   const uint32_t tmem_base = tmem_holder;
   const int rp = (p.R + 15) / 16 * 16, group = 256 / rp, passes = (count + group - 1) / group;
   const int kb0 = p.kblocks * crank / p.split, kb1 = p.kblocks * (crank + 1) / p.split;
+  const int stage_bytes = kOpBytes + min(group, count) * rp * 128, stages = min(low_ring(p.R) / stage_bytes, kLowStagesMax);
   int issued = 0;
 
   if (warp == 0) {
@@ -119,7 +120,7 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         for (int kb = kb0; kb < kb1; kb++, issued++) {
           const int s = issued % stages;
           if (!gemm_wait(empty + s, ((issued / stages) & 1u) ^ 1u, gw, 1)) goto done;
-          uint8_t* at = ring + s * kLowStage;
+          uint8_t* at = ring + s * stage_bytes;
           mbar_arrive_expect(full + s, kOpBytes + n * rp * 128);
           tma_load_2d(at, &map_x, kb * kBlockK, row0, full + s);
           for (int i = 0; i < n; i++) tma_load_2d(at + kOpBytes + i * rp * 128, &map_a, kb * kBlockK, list[ps * group + i] * p.R, full + s);
@@ -138,7 +139,7 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           const int s = it % stages;
           if (!gemm_wait(full + s, (it / stages) & 1u, gw, 3)) goto done;
           tc_fence_after();
-          const uint64_t da = umma_desc_k128(ring + s * kLowStage), db = umma_desc_k128(ring + s * kLowStage + kOpBytes);
+          const uint64_t da = umma_desc_k128(ring + s * stage_bytes), db = umma_desc_k128(ring + s * stage_bytes + kOpBytes);
 #pragma unroll
           for (int k = 0; k < kBlockK / 16; k++) umma_bf16(tmem_base, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc, kb > kb0 || k ? 1u : 0u);
           umma_commit(empty + s);
@@ -282,8 +283,8 @@ __device__ __forceinline__ uint4 ldg16(const uint4* p) {      // volatile: issue
   return r;
 }
 
-// V of few rows: eight ranks of a row per CTA, a warp for each.  Bound by latency: a row of A_a is K numbers, eight loads of every lane in
-// flight.
+// V of few rows: eight ranks of a row per CTA, a warp for each, eight loads of every lane of x and of A_a in flight.  Bound by latency: 64 rows
+// of 48 adapters, K = 2048, rank 16: 4.6 us alone, of which 2.4 are those of a launch that finds no adapters; K = 8192, rank 64: 15 us.
 __global__ void __launch_bounds__(256, 3) few_low_rank_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ a,
                                                            const int* __restrict__ ids, const float* __restrict__ scales, int K, int R, int adapters,
                                                            __nv_bfloat16* __restrict__ v) {
@@ -338,7 +339,7 @@ using namespace fp4ar::layer;
 
 static bool adapters_shape_ok(int M, int N, int K, int R, int adapters) {
   return M >= 0 && N >= 8 && K >= 8 && R >= 8 && R <= 128 && adapters >= 1 && N % 8 == 0 && K % 8 == 0 && R % 8 == 0 &&
-         extents_ok((long long)M + 256, (long long)N + 256) && extents_ok((long long)adapters * N + 256, (long long)M + adapters + 1024) &&
+         extents_ok((long long)M + 256, (long long)N + 256) && extents_ok((long long)adapters * N + 256, (long long)adapters * R + 256) && extents_ok((long long)M + 1024, adapters) &&
          extents_ok(K, 0);
 }
 

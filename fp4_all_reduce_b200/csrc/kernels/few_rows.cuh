@@ -5,6 +5,9 @@
 // others with a long chain of K blocks, so a cluster of up to eight CTAs cuts K: each leaves its FP32 sums in shared memory, and all
 // of them add up a share of the outputs, in the order of the CTAs.  Up to 128 rows two CTAs fit an SM, and one's set-up and sums run
 // under the other's loads (WIDE = false); more rows take groups of up to 256, a CTA for each (WIDE).
+// Bound by the reads of W, by launch and latency where W is small: F = 8192, K = 6144 (201 MB), 16 rows 35 us, 5.8 TB/s; F = 2048 (50 MB), 1 row
+// 11.6 us, 48 rows 13.3 (one CTA per tile, whole K loops: 39 and 40; tiles of 256 rows of x: 28 and 27); N = 6144, K = 2048, rank 16
+// (26 and 38 MB): 1 row 8.6, 64 rows of 48 adapters 14.5.
 //   kGated   the 128 rows are 64 gate rows and the 64 up rows that go with them: their product is taken where the sums meet
 //   kAdapt   the low-rank parts of the outputs that a CTA adds up are computed by the epilogue warps while the weights stream in, by
 //            plain FP32 products with V.  V comes from a launch before this one; only those warps wait for it (see below)
@@ -126,7 +129,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if constexpr (OP == kAdapt) {
       // The low-rank parts of this CTA's share of the outputs, a warp for each row of x.  B_a is read as it lies: `width` lanes have 16
       // bytes each of one of its rows (eight ranks, whose V stay in registers), so a warp's load is 512 contiguous bytes, and the
-      // lanes of a row add up by shuffles.  (A lane with four rows of its own: 41 us instead of 5 at 64 rows, R = 64.)  The lines
+      // lanes of a row add up by shuffles.  (A lane with four rows of its own: 24 us instead of 5 at 64 rows of 16 adapters,
+      // K = 8192, R = 64, where the product alone takes 25.)  The lines
       // are asked for before V is there.
       const int pieces = p.R / 8, width = pieces > 8 ? 16 : pieces > 4 ? 8 : pieces > 2 ? 4 : pieces, per_load = 32 / width;
       const int sub = lane % width, line = (p.R + kChunk - 1) / kChunk * 64;
@@ -318,7 +322,10 @@ int launch_few_rows(const void* w, long rows, const void* x, int K, FewParams p,
   cfg.gridDim = dim3((unsigned)(tiles * p.split));
   cfg.blockDim = dim3(kFewThreads<OP>);
   p.low_offset = p.stages * stage > sums ? p.stages * stage : sums;
-  cfg.dynamicSmemBytes = p.low_offset + lows + 1024;
+  // Never so little that more CTAs fit an SM than its TMEM has columns for: one that waits for columns while its cluster waits for it, and
+  // another the other way round, would wait for ever.
+  const int least = (WIDE ? 116 : 78) * 1024, needed = p.low_offset + lows + 1024;
+  cfg.dynamicSmemBytes = needed > least ? needed : least;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

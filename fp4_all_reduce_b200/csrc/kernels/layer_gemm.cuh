@@ -17,6 +17,10 @@
 //   warps 2-9   epilogue, two per TMEM lane quarter with half of the columns each: tcgen05.ld, activation, BF16, a 32 x 64 slab per
 //               warp in swizzled shared memory, TMA store
 //   warps 10-11 kAdapt: the blocks of low-rank factors
+// Bound by the tensor pipe under the power cap: forward 4096 x 8192, K = 6144: 632 us, 1305 TFLOP/s, where a library product of these
+// sizes without the activation takes 568 - 611; 2048 x 2048, K = 6144: 70 - 73 us (82).  At 4096 x 2048 the pipe is busy for 76 (forward), 82
+// (dx) and 82 % (dW) of the kernel, at 1.54 GHz; a K block takes a pair 0.31 us, about 8 us go to launch, the first loads, the
+// last tile's epilogue and the end.  Calls of one or two waves of tiles leave units idle (1031 x 1368: 55 tiles for 74 units, 42 us).
 // Ragged sizes need no code in the main loop: tensor maps fill with zeros beyond their extents and stores are clipped.
 //
 // MN-major tiles: a box of 64 (outer index, 128 bytes, swizzled) x 64 K rows is 8 KB; a tile of 128 is two boxes.  In the
@@ -38,7 +42,7 @@ namespace layer {
 
 enum : int { kGated = 0, kInput = 1, kWeight = 2, kAdapt = 3 };
 
-constexpr int kRowsCta = 128, kBlockK = 64, kHalf = 128, kStages = 6;
+constexpr int kRowsCta = 128, kBlockK = 64, kStages = 6;
 template <int OP> constexpr int kThreads = OP == kAdapt ? 384 : 320;
 constexpr int kOpBytes = kRowsCta * kBlockK * 2;               // 16 KB of A, 16 KB of B per CTA and stage
 constexpr int kStage = 2 * kOpBytes;

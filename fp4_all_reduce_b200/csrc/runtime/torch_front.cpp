@@ -284,13 +284,18 @@ std::tuple<Tensor, Tensor> op_gated_linear(const Tensor& x, const Tensor& wt, in
   return {std::move(out), std::move(pre)};
 }
 
-std::tuple<Tensor, Tensor> op_gated_backward(const Tensor& dh, const Tensor& pre, const Tensor& x, const Tensor& wt, int64_t act, bool need_dx,
+std::tuple<Tensor, Tensor> op_gated_backward(const Tensor& dh_, const Tensor& pre, const Tensor& x, const Tensor& wt, int64_t act, bool need_dx,
                                              bool need_dw) {
   const GatedShape s(x, wt, act);
   const c10::Device dev = x.device();
+  TORCH_CHECK_VALUE(dh_.dim() == 2 && dh_.size(0) == s.M && dh_.size(1) == s.F, "dh must have shape [", s.M, ", ", s.F, "], got ", shape_text(dh_));
+  require_on(dh_, dev, "dh");
+  const c10::cuda::CUDAGuard guard(dev);
+  // a gradient comes as autograd made it: any strides, any place in its storage
+  Tensor dh = dh_.contiguous();
+  if (reinterpret_cast<uintptr_t>(dh.data_ptr()) & 15) dh = dh.clone();
   require_matrix(dh, at::kBFloat16, {s.M, s.F}, dev, "dh");
   require_matrix(pre, at::kFloat, {s.M, 2 * s.F}, dev, "pre");
-  const c10::cuda::CUDAGuard guard(dev);
   Tensor dx, dw;
   if (!need_dx && !need_dw) return {dx, dw};
   if (need_dx) dx = new_empty({s.M, s.K}, at::kBFloat16, dev);
@@ -312,7 +317,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    auto r = op_gated_backward(grads[0].contiguous(), saved[2], saved[0], saved[1], ctx->saved_data["activation"].toInt(), ctx->needs_input_grad(0),
+    auto r = op_gated_backward(grads[0], saved[2], saved[0], saved[1], ctx->saved_data["activation"].toInt(), ctx->needs_input_grad(0),
                                ctx->needs_input_grad(1));
     torch::autograd::variable_list out{std::move(std::get<0>(r)), std::move(std::get<1>(r))};
     if (at::GradMode::is_enabled()) {            // create_graph: the gradients cannot be differentiated again, and say so
@@ -346,7 +351,7 @@ Tensor op_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, 
   const int64_t n = a.size(0), R = a.size(1);
   TORCH_CHECK_VALUE(n >= 1, "a must hold at least one adapter");
   TORCH_CHECK_VALUE(R >= 8 && R % 8 == 0 && R <= 128, "the rank must be a multiple of 8 up to 128 (pad with zeros), got ", R);
-  require_size(M, "rows"); require_size(K, "K"); require_size(n * Nn, "adapters x N");
+  require_size(M, "rows"); require_size(K, "K"); require_size(n * Nn, "adapters x N"); require_size(n * R, "adapters x R");
   const c10::Device dev = x.device();
   require_matrix(x, at::kBFloat16, {M, K}, dev, "x");
   require_matrix(wt, at::kBFloat16, {Nn, K}, dev, "wt");

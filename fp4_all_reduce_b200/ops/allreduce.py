@@ -209,7 +209,7 @@ def _gated_grad(ctx, dh):
     x, wt = ctx.saved_tensors
     need_dx, need_dw = ctx.needs_input_grad[:2]
     pre = torch.ops.fp4ar.gated_linear_pre(x, wt, ctx.activation)[1]
-    dx, dw = torch.ops.fp4ar.gated_linear_backward(dh.contiguous(), pre, x, wt, ctx.activation, need_dx, need_dw)
+    dx, dw = torch.ops.fp4ar.gated_linear_backward(dh, pre, x, wt, ctx.activation, need_dx, need_dw)
     return dx if need_dx else None, dw if need_dw else None, None
 
 

@@ -38,6 +38,6 @@ def gated_linear_forward(x: torch.Tensor, wt: torch.Tensor, activation: int = N.
 
 def gated_linear_backward(dh: torch.Tensor, pre: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, activation: int = N.ACT_SILU, *,
                           need_dx: bool = True, need_dwt: bool = True) -> tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
-    """(dx, dwt) for the gradient dh of h, each None where it is not needed.  dh may have any strides (an expanded one of a
-    sum's gradient too)."""
-    return N.front().gated_backward(dh.contiguous(), pre, x, wt, activation, need_dx, need_dwt)
+    """(dx, dwt) for the gradient dh of h, each None where it is not needed.  dh may have any strides and any place in
+    its storage."""
+    return N.front().gated_backward(dh, pre, x, wt, activation, need_dx, need_dwt)

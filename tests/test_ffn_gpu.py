@@ -117,6 +117,15 @@ def test_one_input_needs_a_gradient_and_any_layout_of_dh(M):
     _within(a[0], wx, bx), _within(b[1], ww, bw)
 
 
+def test_a_gradient_that_starts_anywhere():
+    x, wt, _ = _data(6, 72, 40, 7)
+    _, pre = ffn.gated_linear_forward(x, wt)
+    room = torch.randn(6 * 40 + 3, device="cuda").to(torch.bfloat16)
+    dh = room[3:].view(6, 40)                                        # contiguous, six bytes behind a boundary
+    a, b = ffn.gated_linear_backward(dh, pre, x, wt), ffn.gated_linear_backward(dh.clone(), pre, x, wt)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_no_second_derivative():
     x, wt, _ = _data(4, 16, 8, 8)
     x.requires_grad_()
@@ -238,6 +247,39 @@ def test_captured_and_replayed(M, K, F):
         torch.cuda.synchronize()
         assert torch.equal(h, h2) and torch.equal(dx, dx2) and torch.equal(dw, dw2)
     assert G.gemm_status().code == 0
+
+
+_FIRST = """
+import torch
+from fp4_all_reduce_b200.ops import adapters, ffn, gemm
+for rows in (4, 300, 1100):
+    x = torch.ones(rows, 4096, device="cuda", dtype=torch.bfloat16)
+    wt = torch.full((4096, 4096), 2.0 ** -12, device="cuda", dtype=torch.bfloat16)
+    a, b = torch.zeros(3, 8, 4096, device="cuda", dtype=torch.bfloat16), torch.ones(3, 4096, 8, device="cuda", dtype=torch.bfloat16)
+    ids = torch.zeros(rows, device="cuda", dtype=torch.int32)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        h, pre = ffn.gated_linear_forward(x, wt)
+        dx, dw = ffn.gated_linear_backward(torch.ones_like(h), pre, x, wt)
+        y = adapters.linear_adapters(x, wt, ids, a, b)
+    g.replay()
+    torch.cuda.synchronize()
+    want = torch.sigmoid(torch.ones(()).double()).item()             # gate = up = 1
+    assert abs(h.double() - want).max().item() <= want * 2 ** -8 and (pre == 1).all() and (y == 1).all()
+    assert gemm.gemm_status().code == 0
+print("captured first")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", _FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and "captured first" in p.stdout, p.stderr[-2000:]
 
 
 def test_calls_on_several_streams_at_once():

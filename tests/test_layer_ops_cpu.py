@@ -64,6 +64,7 @@ def test_the_c_interface_checks_before_it_launches(cuda_lib):
     assert lib.fp4ar_linear_adapters(p, p, None, p, p, None, 4, 16, 16, 8, 2, p, p, None) == 1
     assert lib.fp4ar_linear_adapters(p, p, p, p, p, None, 4, 16, 16, 8, 2, None, p, None) == 1     # workspace
     assert lib.fp4ar_linear_adapters(p, p, p, p, p, None, 4, 8192, 16, 8, 1 << 18, p, p, None) == 1   # adapters x N beyond 32 bits
+    assert lib.fp4ar_linear_adapters(p, p, p, p, p, None, 4, 8, 8, 128, 1 << 25, p, p, None) == 1     # adapters x R beyond 32 bits
     assert lib.fp4ar_linear_adapters(None, None, None, None, None, None, 0, 16, 16, 8, 2, None, None, None) == 0
     # the workspace holds V (two BF16 halves per rank, ranks in blocks of 32) and a list of up to 256 adapters per 256 rows
     assert lib.fp4ar_adapters_workspace(1000, 40, 7) >= 1000 * 64 * 4 + 4 * 257 * 4
