@@ -79,7 +79,7 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   if (warp == 1) { tmem_alloc(&tmem_holder, 256); tmem_relinquish(); }
   GemmWait gw{&abort_flag, p.status, p.timeout_ns};
   pdl_wait_prior_grids();
-  pdl_release_dependents();
+  pdl_release_dependents();                              // after the wait: the product with W relies on it
 
   // the distinct adapters of the 128 rows, in the order of their first rows; thread 64 + r has row r
   auto id_of = [&](int row) {
@@ -256,10 +256,10 @@ static int launch_low_rank(const void* x, const void* a, int K, LowParams p, cud
   p.timeout_ns = kWaitLimitNs;
   CUtensorMap mx, ma;
   if (!map_2d(&mx, x, p.M, K, 128) || !map_2d(&ma, a, (long)p.adapters * p.R, K, (p.R + 15) / 16 * 16)) return FP4AR_ERR_UNSUPPORTED;
-  // as many CTAs per 128 rows, up to eight, as the SMs have room for
-  const int tiles = (p.M + 127) / 128, sms = device_sm_count();
+  // Up to eight CTAs per 128 rows.  Where a quarter of the SMs will do, no more: the product with W starts on the others meanwhile.
+  const int tiles = (p.M + 127) / 128, sms = device_sm_count(), most = 4 * tiles <= sms ? sms / 4 : sms;
   p.split = 1;
-  while (p.split < 8 && 2 * p.split * tiles <= sms && 2 * p.split <= p.kblocks) p.split *= 2;
+  while (p.split < 8 && 2 * p.split * tiles <= most && 2 * p.split <= p.kblocks) p.split *= 2;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(tiles * p.split);

@@ -224,8 +224,8 @@ static __device__ __noinline__ bool low_rank_unsafe(const Params& p, int adapter
 static __device__ __noinline__ float low_rank_dot(const __nv_bfloat16* v, const __nv_bfloat16* b, int R) {
   float s = 0.0f;
   for (int r = 0; r < R; r++) {
-    const __nv_bfloat16* line = v + (r / kChunk) * 64 + r % kChunk;
-    s = fmaf(__bfloat162float(line[0]) + __bfloat162float(line[32]), __bfloat162float(b[r]), s);
+    const unsigned short* line = reinterpret_cast<const unsigned short*>(v) + (r / kChunk) * 64 + r % kChunk;
+    s = fmaf(bf16_lo(__ldcg(line)) + bf16_lo(__ldcg(line + 32)), __bfloat162float(b[r]), s);
   }
   return s;
 }
@@ -280,8 +280,11 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   const uint32_t tmem_base = *tmem_holder;
   GemmWait gw{abort_flag, p.status, p.timeout_ns};
 
-  pdl_wait_prior_grids();
+  // kAdapt: the launch before this one lets it start only after its own wait, so everything before that one is complete here; what that
+  // one itself writes (V, the lists) is waited for by those who read it, behind the K loop of their first tile.
+  if (OP != kAdapt) pdl_wait_prior_grids();
   pdl_release_dependents();
+  auto factors_ready = [&]() { if (OP == kAdapt) pdl_wait_prior_grids(); };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -317,6 +320,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
           }
         }
         if (OP == kAdapt && sg.kind != kProduce) {
+          factors_ready();
           // hand the next stages, as they come free, to the warps that fill them.  (Those cannot wait for `empty` themselves: a parity
           // says nothing to who has not seen every round of a stage.)
           const int blocks = p.lists[(size_t)tm * kListStride] * ((p.R + kChunk - 1) / kChunk);
@@ -350,6 +354,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
           umma_commit_pair(empty + s);
         }
         if (OP == kAdapt && sg.kind != kProduce) {
+          factors_ready();
           int tm, tn;
           tile_at(sg.tile, m_tiles, n_tiles, tm, tn);
           const int* list = p.lists + (size_t)tm * kListStride;
@@ -379,6 +384,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       while (walk.next(sg)) {
         next += (uint32_t)sg.count;
         if (sg.kind == kProduce) continue;
+        factors_ready();
         int tm, tn;
         tile_at(sg.tile, m_tiles, n_tiles, tm, tn);
         const int blocks = p.lists[(size_t)tm * kListStride] * ((p.R + kChunk - 1) / kChunk);
@@ -398,6 +404,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
     for (uint32_t tile_i = 0; walk.next(sg); tile_i++) {
       next += (uint32_t)sg.count;
       if (sg.kind == kProduce) continue;
+      factors_ready();
       int tm, tn;
       tile_at(sg.tile, m_tiles, n_tiles, tm, tn);
       const int m0 = tm * 256 + (int)crank * 128, n0 = tn * 256 + (int)crank * 128;
@@ -520,6 +527,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
         if (OP == kAdapt && sg.kind != kProduce) {
           const int id = mine ? p.ids[row0 + lane] : -1;
           if (unsafe_tile[tile_i % kVerdicts] == tile_i + 1u && id >= 0 && id < p.adapters && low_rank_unsafe(p, id, n0)) {
+            factors_ready();
             slow = id;
             vrow = p.v + (size_t)(row0 + lane) * ((p.R + kChunk - 1) / kChunk * 64);
           }
