@@ -713,9 +713,11 @@ int launch_pair_gemm(const Maps& maps, Params p, cudaStream_t stream) {
   int units = p.cut_units > whole ? p.cut_units : whole;
   std::optional<SplitSpace> space;
   if (p.cut_units) {
-    space.emplace(stream);
-    p.partial = space->partial();
-    p.flags = space->flags();
+    try {
+      space.emplace(stream);
+      p.partial = space->partial();
+      p.flags = space->flags();
+    } catch (...) {}                       // no host memory for it: whole tiles
     if (!p.partial) { p.cut_units = 0; units = whole; }
   }
   cfg.gridDim = dim3(2 * units);
