@@ -281,8 +281,9 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
   GemmWait gw{abort_flag, p.status, p.timeout_ns};
 
   // kAdapt: the launch before this one lets it start only after its own wait, so everything before that one is complete here; what that
-  // one itself writes (V, the lists) is waited for by those who read it, behind the K loop of their first tile.
-  if (OP != kAdapt) pdl_wait_prior_grids();
+  // one itself writes (V, the lists) is waited for by those who read it, behind the K loop of their first tile.  Not where tiles are cut:
+  // another thread may have put a launch with the same slots in between, and that one has to be through.
+  if (OP != kAdapt || p.cut_units) pdl_wait_prior_grids();
   pdl_release_dependents();
   auto factors_ready = [&]() { if (OP == kAdapt) pdl_wait_prior_grids(); };
 
@@ -707,7 +708,7 @@ int launch_pair_gemm(const Maps& maps, Params p, cudaStream_t stream) {
   }
   constexpr int kTileN = OP == kGated ? 128 : 256;
   const long tiles = ((long)p.M + 255) / 256 * (((long)p.N + kTileN - 1) / kTileN);
-  if (tiles > 0x7fffffffL) return FP4AR_ERR_ARGUMENT;
+  if (tiles > 0x7fff0000L) return FP4AR_ERR_ARGUMENT;
   const int whole = tiles < fits ? (int)tiles : fits;
   p.cut_units = cut_units((int)tiles, p.kblocks, fits);
   int units = p.cut_units > whole ? p.cut_units : whole;

@@ -166,6 +166,34 @@ def test_many_calls_in_a_row_give_the_same_bits():
     assert G.gemm_status().code == 0
 
 
+def test_two_threads_on_one_stream():
+    """Launches of two threads interleave on their common stream; the last two shapes cut K loops, whose slots they share."""
+    import threading
+
+    from fp4_all_reduce_b200.ops import ffn
+
+    sets = [_data(m, k, nn, n, 16, 40 + i) for i, (m, k, nn, n) in enumerate(((64, 512, 1032, 9), (600, 512, 1032, 9), (600, 8192, 2048, 3), (1100, 6144, 4096, 5)))]
+    gate = [s[1].repeat(2, 1) for s in sets]
+    want = [AD.linear_adapters(*s) for s in sets]
+    want_h = [ffn.gated_linear(s[0], g) for s, g in zip(sets, gate)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(seed):
+        for i in range(40):
+            j = (i * 7 + seed) % 4
+            y, h = AD.linear_adapters(*sets[j]), ffn.gated_linear(sets[j][0], gate[j])
+            if not (torch.equal(y, want[j]) and torch.equal(h, want_h[j])):
+                bad.append((seed, i, j))
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and G.gemm_status().code == 0, bad
+
+
 def test_refusals():
     x, wt, ids, a, b, sc = _data(4, 16, 24, 3, 8)
     ok = dict(x=x, wt=wt, ids=ids, a=a, b=b, scales=sc)
