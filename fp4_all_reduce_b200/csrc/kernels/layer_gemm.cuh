@@ -650,21 +650,17 @@ done:
 // ---- host side ----
 // A BF16 matrix of `rows` rows, `cols` contiguous columns; box of 64 columns x box_rows.
 inline bool map_2d(CUtensorMap* m, const void* base, long rows, long cols, int box_rows) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)cols * 2};
   const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, one[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 // [rows][2][cols] FP32: the two projections of every row, each clipped at its own width
 inline bool map_pre(CUtensorMap* m, const void* base, long rows, long cols) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return false;
   const cuuint64_t dims[3] = {(cuuint64_t)cols, 2, (cuuint64_t)rows}, strides[2] = {(cuuint64_t)cols * 4, (cuuint64_t)cols * 8};
   const cuuint32_t box[3] = {32, 1, 32}, one[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;

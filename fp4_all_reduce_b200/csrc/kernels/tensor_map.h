@@ -23,5 +23,15 @@ inline EncodeTiledFn encode_tiled_fn() {
   });
   return fn;
 }
+// Encodes a map.  The driver's function wants a context that is current to the calling thread, which a thread whose first CUDA call this
+// is does not have yet; cudaSetDevice makes it so (during a capture too).
+template <class... A>
+bool encode_tiled(A... args) {
+  const EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return false;
+  if (fn(args...) == CUDA_SUCCESS) return true;
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && fn(args...) == CUDA_SUCCESS;
+}
 
 }  // namespace fp4ar

@@ -166,6 +166,33 @@ def test_many_calls_in_a_row_give_the_same_bits():
     assert G.gemm_status().code == 0
 
 
+@pytest.mark.parametrize("which", ["few rows", "tiles", "gated", "NVFP4"])
+def test_the_first_cuda_call_of_a_thread(which):
+    """A new thread has no context of its own yet when the tensor maps are made."""
+    import threading
+
+    from fp4_all_reduce_b200.ops import ffn
+
+    s = _data(40 if which == "few rows" else 700, 256, 512, 3, 16, 8)
+    call = {"gated": lambda: ffn.gated_linear(s[0], s[1]), "NVFP4": lambda: G.gemm_nvfp4(s[0], s[1], 1.0)}.get(which, lambda: AD.linear_adapters(*s))
+    want = call()
+    del want                                        # (its memory serves the thread's call: nothing there but the launch needs CUDA)
+    want, got = call(), []
+    spare = call()
+    del spare
+
+    def work():
+        try:
+            got.append(call())
+        except Exception as e:
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert torch.is_tensor(got[0]) and torch.equal(got[0], want), got
+
+
 def test_two_threads_on_one_stream():
     """Launches of two threads interleave on their common stream; the last two shapes cut K loops, whose slots they share."""
     import threading
@@ -180,11 +207,14 @@ def test_two_threads_on_one_stream():
     bad = []
 
     def work(seed):
-        for i in range(40):
-            j = (i * 7 + seed) % 4
-            y, h = AD.linear_adapters(*sets[j]), ffn.gated_linear(sets[j][0], gate[j])
-            if not (torch.equal(y, want[j]) and torch.equal(h, want_h[j])):
-                bad.append((seed, i, j))
+        try:
+            for i in range(40):
+                j = (i * 7 + seed) % 4
+                y, h = AD.linear_adapters(*sets[j]), ffn.gated_linear(sets[j][0], gate[j])
+                if not (torch.equal(y, want[j]) and torch.equal(h, want_h[j])):
+                    bad.append((seed, i, j))
+        except Exception as e:
+            bad.append((seed, e))
 
     threads = [threading.Thread(target=work, args=(s,)) for s in range(3)]
     for t in threads:
