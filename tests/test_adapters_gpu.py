@@ -33,7 +33,7 @@ def _check(args):
                                         (33, 1992, 328, 40, 16), (64, 2048, 512, 48, 16), (65, 64, 64, 70, 32), (100, 256, 200, 7, 128),
                                         (128, 320, 256, 1, 40), (129, 136, 520, 9, 48), (255, 1000, 136, 300, 16), (257, 264, 264, 12, 72),
                                         (700, 512, 1032, 6, 104), (1031, 200, 648, 16, 32), (2050, 128, 1160, 3, 64),
-                                        (1500, 72, 136, 900, 8), (600, 256, 264, 700, 128), (513, 320, 520, 513, 40), (300, 6144, 264, 4, 16)])
+                                        (1500, 72, 136, 900, 8), (600, 256, 264, 700, 128), (513, 320, 520, 513, 40), (300, 6144, 264, 4, 16), (100000, 16, 8, 5, 8), (7, 32768, 16, 3, 32), (2, 64, 100000, 4, 16)])
 def test_mixed_rows(M, K, Nn, n, r):
     _check(_data(M, K, Nn, n, r))
 

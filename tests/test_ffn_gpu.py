@@ -28,7 +28,7 @@ def _within(got, want, bound, dtype=torch.bfloat16):
 SHAPES = [(1, 8, 8), (1, 64, 64), (2, 520, 72), (7, 1024, 136), (16, 2048, 256), (17, 72, 1000), (33, 200, 128), (63, 1000, 520),
           (64, 256, 264), (65, 6144, 64), (127, 128, 8), (128, 192, 128), (129, 4104, 200), (255, 136, 1368), (256, 64, 320), (257, 320, 136),
           (385, 2048, 512), (1031, 264, 648), (2050, 128, 1160), (500, 512, 264), (900, 136, 72),
-          (1024, 256, 136), (400, 128, 4104)]
+          (1024, 256, 136), (400, 128, 4104), (200000, 8, 8), (1, 64, 100000), (3, 32768, 16)]
 
 
 @pytest.mark.parametrize("act", [0, 1, 2])
@@ -290,7 +290,7 @@ def test_calls_on_several_streams_at_once():
         h, pre = ffn.gated_linear_forward(x, wt)
         want.append((h, *ffn.gated_linear_backward(dh, pre, x, wt)))
     torch.cuda.synchronize()
-    streams = [torch.cuda.Stream() for _ in range(6)]
+    streams = [torch.cuda.Stream() for _ in range(11)]           # more than have a workspace of their own
     got = []
     for r in range(4):
         for i, s in enumerate(streams):
