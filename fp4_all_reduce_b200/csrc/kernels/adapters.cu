@@ -2,6 +2,8 @@
 //
 // Two launches: a first kernel computes V[i] = s_a x_i A_a^T and lists the adapters of every 256 rows; the product with W then takes
 // V_a B_a^T into the same accumulators (layer_gemm.cuh).
+#include <algorithm>
+
 #include "few_rows.cuh"
 #include "layer_gemm.cuh"
 
@@ -38,7 +40,8 @@ struct LowParams {
 // time is that of reading x.  A cluster of `split` CTAs cuts K where there are few rows; their sums meet in shared memory, in the
 // order of the CTAs.
 // The ring's stages are as large as the adapters of the rows need (8192 x 8192, rank 64: four stages for 256 rows of A 42 us, eight for one
-// adapter 38, which is 151 MB at 4.0 TB/s, launch, lists and the exchange of the sums, about 5 us, included; 4096 x 2048, rank 16: 12 us).
+// adapter 36, which is 151 MB at 4.2 TB/s, launch, lists and the exchange of the sums, about 5 us, included; 4096 x 2048, rank 16, two CTAs
+// for 128 rows: 13 us.)
 constexpr int kLowStagesMax = 10;
 __host__ __device__ constexpr int low_ring(int R) { return (R <= 64 ? 4 : 3) * (kOpBytes + 256 * kBlockK * 2); }
 __host__ __device__ constexpr int low_smem(int R) { return low_ring(R) + 128 * R * 4 + 1024; }
@@ -62,9 +65,10 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   __shared__ uint32_t tmem_holder;
   __shared__ volatile uint32_t abort_flag;
   __shared__ __align__(16) int sid[256];
-  __shared__ int list[128], scount[4], scount2[4], count;
+  __shared__ int list[128], wcount[4], scount[4], scount2[4], count;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* part = reinterpret_cast<float*>(ring + low_ring(p.R));            // [128][R]
+  float* scale = reinterpret_cast<float*>(ring);                           // [128], behind the last product
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tile = blockIdx.x / p.split, crank = blockIdx.x % p.split, row0 = tile * 128;
   if (tid == 0) {
@@ -90,12 +94,21 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   int id = -1;
   bool first = false;
   uint32_t votes = 0;
-  if (r >= 0) sid[r] = id = id_of(row0 + r);
+  int* const firsts = sid + 128;                         // those of each warp's rows; the list of 256 rows overwrites them later
+  if (r >= 0) {
+    sid[r] = id = id_of(row0 + r);
+    const uint32_t same = __match_any_sync(0xffffffffu, id);
+    first = id >= 0 && lane == __ffs(same) - 1;
+    votes = __ballot_sync(0xffffffffu, first);
+    if (first) firsts[(warp - 2) * 32 + __popc(votes & ((1u << lane) - 1u))] = id;
+    if (lane == 0) wcount[warp - 2] = __popc(votes);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (r >= 0) {
-    first = id >= 0 && !seen_before(sid, r, id);
+    for (int w = 0; w < warp - 2; w++)
+      for (int i = 0; i < wcount[w]; i++) first = first && firsts[w * 32 + i] != id;
     votes = __ballot_sync(0xffffffffu, first);
     if (lane == 0) scount[warp - 2] = __popc(votes);
   }
@@ -168,6 +181,7 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     // TMEM lane quarter warp & 3 has rows 32 (warp & 3) ...
     const int q = warp & 3, row = q * 32 + lane;
     const int mine = sid[row];
+    const float factor = mine >= 0 && p.scales ? p.scales[mine] : 1.0f;
     for (int ps = 0; ps < passes; ps++) {
       if (!__all_sync(0xffffffffu, gemm_wait(&acc_full, ps & 1u, gw, 4))) break;
       tc_fence_after();
@@ -192,6 +206,7 @@ low_rank_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty);
     }
+    scale[row] = factor;                                 // the last product is through with the ring
   }
 done:
   tc_fence_before();
@@ -208,31 +223,35 @@ done:
     __syncthreads();
   }
   if (p.split > 1) cluster_sync_all();
-  // this CTA's share of the rows: the sum of the cluster's parts, scaled, as two BF16 halves
-  const int share = 128 / p.split, padded = (p.R + kChunk - 1) / kChunk * kChunk;
-  for (int i = tid; i < share * (padded / 2); i += 192) {
-    const int rr = crank * share + i / (padded / 2), n = i % (padded / 2) * 2;
-    const int a = sid[rr];
-    if (a < 0) continue;                                 // nobody reads its V
-    float2 s = make_float2(0.0f, 0.0f);
+  // this CTA's share of the rows: the sum of the cluster's parts, scaled, as two BF16 halves; four columns of a row per thread
+  const int share = 128 / p.split, padded = (p.R + kChunk - 1) / kChunk * kChunk, per_row = padded / 4, rows = 32 / per_row;
+  const int n = lane % per_row * 4;
+  for (int i = warp * rows + lane / per_row; i < share && lane < rows * per_row; i += 6 * rows) {
+    const int rr = crank * share + i;
+    if (sid[rr] < 0) continue;                           // nobody reads its V
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (n < p.R) {
-      for (int d = 0; d < p.split; d++) {
-        float2 f;
-        if (p.split > 1)
-          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(cluster_addr(part + rr * p.R + n, d)));
-        else
-          f = *reinterpret_cast<const float2*>(part + rr * p.R + n);
-        s.x += f.x;
-        s.y += f.y;
+      if (p.split == 1) {
+        s = *reinterpret_cast<const float4*>(part + rr * p.R + n);
+      } else {
+        float4 f[8];                                     // all of them in flight
+#pragma unroll
+        for (int d = 0; d < 8; d++)
+          if (d < p.split) f[d] = cluster_ld4(cluster_addr(part + rr * p.R + n, d));
+#pragma unroll
+        for (int d = 0; d < 8; d++)
+          if (d < p.split) { s.x += f[d].x; s.y += f[d].y; s.z += f[d].z; s.w += f[d].w; }
       }
-      if (p.scales) { const float sc = p.scales[a]; s.x *= sc; s.y *= sc; }
+      const float sc = scale[rr];
+      s.x *= sc; s.y *= sc; s.z *= sc; s.w *= sc;
     }
     // the rounded value and what the rounding left; what is not finite stays in the first alone
-    const uint32_t hi = pack_bf16(s.x, s.y);
-    const float l0 = s.x - bf16_lo(hi), l1 = s.y - bf16_hi(hi);
-    uint32_t* line = reinterpret_cast<uint32_t*>(p.v + (size_t)(row0 + rr) * (2 * padded) + n / kChunk * 64 + n % kChunk);
-    line[0] = hi;
-    line[kChunk / 2] = pack_bf16(fabsf(l0) <= 3.4e38f ? l0 : 0.0f, fabsf(l1) <= 3.4e38f ? l1 : 0.0f);
+    auto left = [](float v, float rounded) { const float l = v - rounded; return fabsf(l) <= 3.4e38f ? l : 0.0f; };
+    const uint2 hi = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+    __nv_bfloat16* line = p.v + (size_t)(row0 + rr) * (2 * padded) + n / kChunk * 64 + n % kChunk;
+    *reinterpret_cast<uint2*>(line) = hi;
+    *reinterpret_cast<uint2*>(line + kChunk) = make_uint2(pack_bf16(left(s.x, bf16_lo(hi.x)), left(s.y, bf16_hi(hi.x))),
+                                                          pack_bf16(left(s.z, bf16_lo(hi.y)), left(s.w, bf16_hi(hi.y))));
   }
   if (p.split > 1) cluster_sync_relaxed();               // a CTA's part is read until here
   if (warp == 1) {
@@ -256,8 +275,10 @@ static int launch_low_rank(const void* x, const void* a, int K, LowParams p, cud
   p.timeout_ns = kWaitLimitNs;
   CUtensorMap mx, ma;
   if (!map_2d(&mx, x, p.M, K, 128) || !map_2d(&ma, a, (long)p.adapters * p.R, K, (p.R + 15) / 16 * 16)) return FP4AR_ERR_UNSUPPORTED;
-  // Up to eight CTAs per 128 rows.  Where a quarter of the SMs will do, no more: the product with W starts on the others meanwhile.
-  const int tiles = (p.M + 127) / 128, sms = device_sm_count(), most = 4 * tiles <= sms ? sms / 4 : sms;
+  // Up to eight CTAs per 128 rows.  Where a quarter of the SMs will do, no more: the product with W starts on the others meanwhile, and there
+  // V is to be ready when its first tiles are.  But two at least, since one takes longer than the tile (4096 x 2048 rows, N = 6144, all:
+  // 105 us with one, 98.5 with two; 1031 x 1992 with 36 CTAs 41, with 72 or 144 43.5).
+  const int tiles = (p.M + 127) / 128, sms = device_sm_count(), most = 4 * tiles <= sms ? std::max(sms / 4, 2 * tiles) : sms;
   p.split = 1;
   while (p.split < 8 && 2 * p.split * tiles <= most && 2 * p.split <= p.kblocks) p.split *= 2;
   cudaLaunchConfig_t cfg;
