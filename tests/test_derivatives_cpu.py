@@ -1,0 +1,68 @@
+"""Derivatives that the feed-forward ops do not have are refused, on meta tensors and, where the refusal comes before the checks of the
+device, on CPU tensors: nothing is dropped in silence."""
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def ops(cuda_lib):
+    from fp4_all_reduce_b200 import _native as N
+    from fp4_all_reduce_b200.ops import allreduce  # noqa: F401  (registers torch.ops.fp4ar)
+
+    try:
+        N.front()
+    except RuntimeError as e:
+        pytest.skip(str(e))
+    return torch.ops.fp4ar
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("needs", ["x", "wt", "both"])
+def test_the_custom_op_has_no_second_derivative(ops, needs):
+    """A loss with a gradient penalty: its backward pass raises, whichever input the gradient is taken of."""
+    x, wt = _meta(5, 16), _meta(48, 16)
+    wanted = {"x": [x], "wt": [wt], "both": [x, wt]}[needs]
+    for t in wanted:
+        t.requires_grad_()
+    h = ops.gated_linear(x, wt, 0)
+    grads = torch.autograd.grad(h.sum(), wanted, create_graph=True)
+    assert [g.shape for g in grads] == [t.shape for t in wanted]
+    loss = h.sum() + sum(g.square().sum() for g in grads)
+    with pytest.raises(RuntimeError, match="gated_linear cannot be differentiated twice"):
+        loss.backward()
+    assert x.grad is None and wt.grad is None
+
+
+def test_a_gradient_of_the_gradient_of_h_is_refused_too(ops):
+    x, wt, dh = _meta(5, 16).requires_grad_(), _meta(48, 16), _meta(5, 24).requires_grad_()
+    (dx,) = torch.autograd.grad(ops.gated_linear(x, wt, 0), x, dh, create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+        torch.autograd.grad(dx.sum(), dh)
+
+
+def test_the_parts_of_the_backward_pass_have_no_gradient_of_their_own(ops):
+    x, wt = _meta(5, 16).requires_grad_(), _meta(48, 16)
+    h, pre = ops.gated_linear_pre(x, wt, 0)
+    for out in (h, pre):
+        with pytest.raises(RuntimeError, match="gated_linear_pre records no gradient"):
+            torch.autograd.grad(out.sum(), x, retain_graph=True)
+    dx, dw = ops.gated_linear_backward(_meta(5, 24), pre.detach(), x, wt, 0, True, True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+        (dx.sum() + dw.sum()).backward()
+
+
+def test_first_gradients_of_the_custom_op_stay(ops):
+    x, wt = _meta(5, 16).requires_grad_(), _meta(48, 16).requires_grad_()
+    ops.gated_linear(x, wt, 0).sum().backward()
+    assert x.grad.shape == x.shape and wt.grad.shape == wt.shape
+    assert not x.grad.requires_grad and not wt.grad.requires_grad
+
+
+def test_a_compiled_step_still_traces(ops):
+    x, wt = _meta(5, 16).requires_grad_(), _meta(48, 16).requires_grad_()
+    h = torch.compile(lambda a, b: ops.gated_linear(a, b, 1), fullgraph=True, backend="aot_eager")(x, wt)
+    dx, dw = torch.autograd.grad(h.sum(), (x, wt))
+    assert dx.shape == x.shape and dw.shape == wt.shape

@@ -1,0 +1,27 @@
+"""Derivatives that the feed-forward ops do not have are refused on the GPU as on the host, those they have stay as they were."""
+import pytest
+import torch
+
+from fp4_all_reduce_b200.ops import allreduce as A  # noqa: F401  (registers torch.ops.fp4ar)
+from fp4_all_reduce_b200.ops import ffn
+
+pytestmark = pytest.mark.gpu
+
+
+def _bf16(*shape, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda").to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("gated", [ffn.gated_linear, lambda x, wt: torch.ops.fp4ar.gated_linear(x, wt, 0)], ids=["ffn", "op"])
+@pytest.mark.parametrize("rows", [4, 300])
+def test_a_gradient_penalty_raises(gated, rows):
+    """First gradients taken with create_graph=True are those taken without; differentiating them raises."""
+    x, wt = _bf16(rows, 16).requires_grad_(), _bf16(48, 16, seed=1).requires_grad_()
+    want = torch.autograd.grad(gated(x, wt).sum(), (x, wt))
+    h = gated(x, wt)
+    grads = torch.autograd.grad(h.sum(), (x, wt), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+    with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+        (h.sum() + grads[0].square().sum()).backward()
+    assert x.grad is None and wt.grad is None
