@@ -342,6 +342,9 @@ Tensor op_gated_linear_auto(const Tensor& x, const Tensor& wt, int64_t act, Tens
   return GatedLinear::apply(x, wt, act);
 }
 
+void require_no_recording(std::initializer_list<const Tensor*> ts) {
+  if (recording(ts)) throw std::runtime_error("linear_adapters has no backward pass: call it under torch.no_grad() or on detached tensors");
+}
 Tensor op_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, const Tensor& a, const Tensor& b, const Tensor& scales, Tensor out) {
   TORCH_CHECK_VALUE(x.dim() == 2, "x must have shape [rows, K], got ", shape_text(x));
   TORCH_CHECK_VALUE(wt.dim() == 2 && wt.size(1) == x.size(1), "wt must have shape [N, ", x.size(1), "], got ", shape_text(wt));
@@ -399,6 +402,15 @@ std::tuple<Tensor, Tensor> lib_gated_linear_backward(const Tensor& dh, const Ten
 }
 Tensor lib_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, const Tensor& a, const Tensor& b, const std::optional<Tensor>& scales) {
   return op_linear_adapters(x, wt, ids, a, b, scales ? *scales : Tensor(), Tensor());
+}
+// Its autograd kernel, on every device: without one torch's fallback would record the call and deliver no gradient.
+Tensor lib_linear_adapters_autograd(c10::DispatchKeySet keys, const Tensor& x, const Tensor& wt, const Tensor& ids, const Tensor& a, const Tensor& b,
+                                    const std::optional<Tensor>& scales) {
+  const Tensor none;
+  require_no_recording({&x, &wt, &a, &b, scales ? &*scales : &none});
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fp4ar::linear_adapters", "").typed<decltype(lib_linear_adapters)>();
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.redispatch(keys & c10::after_autograd_keyset, x, wt, ids, a, b, scales);
 }
 
 // ---- Python entry points: positional arguments only, the wrappers fill in the defaults ----
@@ -572,8 +584,7 @@ PyObject* py_linear_adapters(PyObject*, PyObject* const* p, Py_ssize_t n) {
                &b = tensor_arg(p[4], "b");
   const Tensor scales = p[5] == Py_None ? Tensor() : tensor_arg(p[5], "scales");
   Tensor out = p[6] == Py_None ? Tensor() : tensor_arg(p[6], "out");
-  if (recording({&x, &wt, &a, &b, &scales}))
-    throw std::runtime_error("linear_adapters has no backward pass: call it under torch.no_grad() or on detached tensors");
+  require_no_recording({&x, &wt, &a, &b, &scales});
   return THPVariable_Wrap([&] { NoGil g; return op_linear_adapters(x, wt, ids, a, b, scales, std::move(out)); }());
   END_HANDLE_TH_ERRORS
 }
@@ -758,6 +769,7 @@ TORCH_LIBRARY_IMPL(fp4ar, CUDA, m) {
   m.impl("gated_linear_backward", lib_gated_linear_backward);
   m.impl("linear_adapters", lib_linear_adapters);
 }
+TORCH_LIBRARY_IMPL(fp4ar, Autograd, m) { m.impl("linear_adapters", TORCH_FN(lib_linear_adapters_autograd)); }
 
 PyMODINIT_FUNC PyInit__fp4ar_front() {
   ctx_type.tp_name = "_fp4ar_front.Context";

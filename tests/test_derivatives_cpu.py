@@ -66,3 +66,30 @@ def test_a_compiled_step_still_traces(ops):
     h = torch.compile(lambda a, b: ops.gated_linear(a, b, 1), fullgraph=True, backend="aot_eager")(x, wt)
     dx, dw = torch.autograd.grad(h.sum(), (x, wt))
     assert dx.shape == x.shape and dw.shape == wt.shape
+
+
+def _adapter_tensors(make):
+    return dict(x=make(5, 16), wt=make(48, 16), ids=torch.zeros(5, dtype=torch.int32, device=make(1).device), a=make(2, 8, 16), b=make(2, 48, 8),
+                scales=make(2, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("name", ["x", "wt", "a", "b", "scales"])
+def test_the_op_with_adapters_has_no_backward_pass(ops, name):
+    """As the function in ops/adapters.py, the op refuses the call; without a recording it takes the same tensors."""
+    t = _adapter_tensors(_meta)
+    t[name].requires_grad_()
+    with pytest.raises(RuntimeError, match="linear_adapters has no backward pass"):
+        ops.linear_adapters(**t)
+    with torch.no_grad():
+        y = ops.linear_adapters(**t)
+    assert y.shape == (5, 48) and not y.requires_grad
+    t[name] = t[name].detach()
+    assert not ops.linear_adapters(**t).requires_grad
+
+
+def test_a_compiled_call_with_adapters(ops):
+    t = _adapter_tensors(_meta)
+    fn = torch.compile(lambda *a: ops.linear_adapters(*a), fullgraph=True, backend="aot_eager")
+    assert fn(*t.values()).shape == (5, 48)
+    with pytest.raises(RuntimeError, match="linear_adapters has no backward pass"):
+        fn(t["x"].clone().requires_grad_(), *list(t.values())[1:])

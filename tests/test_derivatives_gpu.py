@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from fp4_all_reduce_b200.ops import adapters as AD
 from fp4_all_reduce_b200.ops import allreduce as A  # noqa: F401  (registers torch.ops.fp4ar)
 from fp4_all_reduce_b200.ops import ffn
 
@@ -25,3 +26,21 @@ def test_a_gradient_penalty_raises(gated, rows):
     with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
         (h.sum() + grads[0].square().sum()).backward()
     assert x.grad is None and wt.grad is None
+
+
+@pytest.mark.parametrize("rows", [4, 600])
+def test_adapters_refuse_a_recording_by_both_entries(rows):
+    x, wt, a, b = _bf16(rows, 64), _bf16(48, 64, seed=1), _bf16(2, 8, 64, seed=2), _bf16(2, 48, 8, seed=3)
+    ids = (torch.arange(rows, device="cuda") % 3).to(torch.int32)
+    scales = torch.full((2,), 0.5, device="cuda")
+    want = AD.linear_adapters(x, wt, ids, a, b, scales)
+    assert torch.equal(torch.ops.fp4ar.linear_adapters(x, wt, ids, a, b, scales), want)
+    for call in (AD.linear_adapters, torch.ops.fp4ar.linear_adapters):
+        for i in (0, 1, 3, 4, 5):
+            args = [x, wt, ids, a, b, scales]
+            args[i] = args[i].clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="linear_adapters has no backward pass"):
+                call(*args)
+            with torch.no_grad():
+                y = call(*args)
+            assert torch.equal(y, want) and not y.requires_grad
