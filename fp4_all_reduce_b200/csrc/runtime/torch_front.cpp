@@ -252,6 +252,12 @@ void require_apart(const Tensor& out, const Tensor& in, const char* name) {
 // Rows and columns as the C interface takes them: 32-bit, with room for a tile.
 void require_size(int64_t n, const char* name) { TORCH_CHECK_VALUE(n <= 0x7fff0000, name, " is too large: ", n); }
 
+// A tangent that a kernel does not see would be lost: torch takes a result without one as constant.
+void require_no_tangent(std::initializer_list<const Tensor*> ts, const char* op) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(std::string(op) + " has no forward-mode derivative");
+}
+
 struct GatedShape {
   int64_t M, K, F;
   GatedShape(const Tensor& x, const Tensor& wt, int64_t act) {
@@ -268,6 +274,7 @@ struct GatedShape {
 };
 
 std::tuple<Tensor, Tensor> op_gated_linear(const Tensor& x, const Tensor& wt, int64_t act, bool want_pre, Tensor out) {
+  require_no_tangent({&x, &wt, &out}, "gated_linear");
   const GatedShape s(x, wt, act);
   const c10::Device dev = x.device();
   if (out.defined()) {
@@ -286,6 +293,7 @@ std::tuple<Tensor, Tensor> op_gated_linear(const Tensor& x, const Tensor& wt, in
 
 std::tuple<Tensor, Tensor> op_gated_backward(const Tensor& dh_, const Tensor& pre, const Tensor& x, const Tensor& wt, int64_t act, bool need_dx,
                                              bool need_dw) {
+  require_no_tangent({&dh_, &pre, &x, &wt}, "gated_linear");
   const GatedShape s(x, wt, act);
   const c10::Device dev = x.device();
   TORCH_CHECK_VALUE(dh_.dim() == 2 && dh_.size(0) == s.M && dh_.size(1) == s.F, "dh must have shape [", s.M, ", ", s.F, "], got ", shape_text(dh_));
@@ -338,6 +346,7 @@ bool recording(std::initializer_list<const Tensor*> ts) {
 // h, recorded where autograd records
 Tensor op_gated_linear_auto(const Tensor& x, const Tensor& wt, int64_t act, Tensor out) {
   if (!recording({&x, &wt})) return std::get<0>(op_gated_linear(x, wt, act, false, std::move(out)));
+  require_no_tangent({&x, &wt}, "gated_linear");            // (forward mode is off inside the recorded function)
   TORCH_CHECK_VALUE(!out.defined(), "out cannot be given where a gradient is recorded");
   return GatedLinear::apply(x, wt, act);
 }
@@ -346,6 +355,7 @@ void require_no_recording(std::initializer_list<const Tensor*> ts) {
   if (recording(ts)) throw std::runtime_error("linear_adapters has no backward pass: call it under torch.no_grad() or on detached tensors");
 }
 Tensor op_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, const Tensor& a, const Tensor& b, const Tensor& scales, Tensor out) {
+  require_no_tangent({&x, &wt, &a, &b, &scales, &out}, "linear_adapters");
   TORCH_CHECK_VALUE(x.dim() == 2, "x must have shape [rows, K], got ", shape_text(x));
   TORCH_CHECK_VALUE(wt.dim() == 2 && wt.size(1) == x.size(1), "wt must have shape [N, ", x.size(1), "], got ", shape_text(wt));
   const int64_t M = x.size(0), K = x.size(1), Nn = wt.size(0);
@@ -409,8 +419,15 @@ Tensor lib_linear_adapters_autograd(c10::DispatchKeySet keys, const Tensor& x, c
   const Tensor none;
   require_no_recording({&x, &wt, &a, &b, scales ? &*scales : &none});
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fp4ar::linear_adapters", "").typed<decltype(lib_linear_adapters)>();
-  const at::AutoDispatchBelowADInplaceOrView below;
+  const at::AutoDispatchBelowAutograd below;
   return op.redispatch(keys & c10::after_autograd_keyset, x, wt, ids, a, b, scales);
+}
+// Between autograd and the kernels of any device, for the ops above: no tangent gets past here.
+void lib_refuse_tangents(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  for (size_t n = op.schema().arguments().size(), i = stack->size() - n; i < stack->size(); i++)
+    if ((*stack)[i].isTensor()) require_no_tangent({&(*stack)[i].toTensor()}, op.schema().name().c_str() + sizeof("fp4ar::") - 1);
+  const at::AutoDispatchBelowADInplaceOrView below;
+  op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
 }
 
 // ---- Python entry points: positional arguments only, the wrappers fill in the defaults ----
@@ -768,6 +785,10 @@ TORCH_LIBRARY_IMPL(fp4ar, CUDA, m) {
   m.impl("gated_linear_pre", lib_gated_linear_pre);
   m.impl("gated_linear_backward", lib_gated_linear_backward);
   m.impl("linear_adapters", lib_linear_adapters);
+}
+TORCH_LIBRARY_IMPL(fp4ar, ADInplaceOrView, m) {
+  for (const char* op : {"gated_linear", "gated_linear_pre", "gated_linear_backward", "linear_adapters"})
+    m.impl(op, torch::CppFunction::makeFromBoxedFunction<&lib_refuse_tangents>());
 }
 TORCH_LIBRARY_IMPL(fp4ar, Autograd, m) { m.impl("linear_adapters", TORCH_FN(lib_linear_adapters_autograd)); }
 

@@ -93,3 +93,56 @@ def test_a_compiled_call_with_adapters(ops):
     assert fn(*t.values()).shape == (5, 48)
     with pytest.raises(RuntimeError, match="linear_adapters has no backward pass"):
         fn(t["x"].clone().requires_grad_(), *list(t.values())[1:])
+
+
+def _forward_mode(fn, args, i):
+    """fn(*args) with a tangent on argument i."""
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        args = list(args)
+        args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+        return fn(*args)
+
+
+def test_the_functions_have_no_forward_mode(ops):
+    """A dual tensor that requires no gradient would pass every other check; the result would have no tangent, which torch takes as zero."""
+    from fp4_all_reduce_b200.ops import adapters, ffn
+
+    def make(*shape, dtype=torch.bfloat16):
+        return torch.zeros(*shape, dtype=dtype)
+
+    x, wt, h, pre = make(5, 16), make(48, 16), make(5, 24), make(5, 48, dtype=torch.float32)
+    t = list(_adapter_tensors(make).values())
+    for name, fn, args, which in (("gated_linear", ffn.gated_linear, (x, wt), (0, 1)), ("gated_linear", ffn.gated_linear_forward, (x, wt), (0, 1)),
+                                  ("gated_linear", ffn.gated_linear_backward, (h, pre, x, wt), (0, 1, 2, 3)),
+                                  ("linear_adapters", adapters.linear_adapters, t, (0, 1, 3, 4, 5))):
+        for i in which:
+            with pytest.raises(RuntimeError, match=f"{name} has no forward-mode derivative"):
+                _forward_mode(fn, args, i)
+        with pytest.raises(ValueError, match="CUDA"):                # as before without a tangent
+            fn(*args)
+    with pytest.raises(RuntimeError, match="gated_linear has no forward-mode derivative"):
+        _forward_mode(lambda a, b: ffn.gated_linear(a, b.requires_grad_()), (x, wt), 0)
+    with pytest.raises(RuntimeError, match="gated_linear has no forward-mode derivative"):
+        torch.func.jvp(lambda a: ffn.gated_linear(a, wt.detach()), (x,), (x,))
+
+
+def test_the_custom_ops_have_no_forward_mode(ops):
+    x, wt, h, pre = _meta(5, 16), _meta(48, 16), _meta(5, 24), _meta(5, 48, dtype=torch.float32)
+    t = list(_adapter_tensors(_meta).values())
+    for name, fn, args, which in (("gated_linear", lambda *a: ops.gated_linear(*a, 0), (x, wt), (0, 1)),
+                                  ("gated_linear_pre", lambda *a: ops.gated_linear_pre(*a, 0), (x, wt), (0, 1)),
+                                  ("gated_linear_backward", lambda *a: ops.gated_linear_backward(*a, 0, True, True), (h, pre, x, wt), (0, 1, 2, 3)),
+                                  ("linear_adapters", ops.linear_adapters, t, (0, 1, 3, 4, 5))):
+        for i in which:
+            for recording in (True, False):
+                with torch.set_grad_enabled(recording), pytest.raises(RuntimeError, match=f"{name} has no forward-mode derivative"):
+                    _forward_mode(fn, args, i)
+        fn(*args)
+    with pytest.raises(RuntimeError):                                # recorded too: torch's own refusal
+        _forward_mode(lambda a, b: ops.gated_linear(a, b.clone().requires_grad_(), 0), (x, wt), 0)
+    # forward over reverse: the tangent of h's gradient does not get lost
+    g = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError):
+        _forward_mode(lambda d: torch.autograd.grad(ops.gated_linear(g, wt, 0), g, d), (h,), 0)

@@ -44,3 +44,27 @@ def test_adapters_refuse_a_recording_by_both_entries(rows):
             with torch.no_grad():
                 y = call(*args)
             assert torch.equal(y, want) and not y.requires_grad
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+
+    x, wt, a, b = _bf16(4, 64), _bf16(48, 64, seed=1), _bf16(2, 8, 64, seed=2), _bf16(2, 48, 8, seed=3)
+    ids = torch.zeros(4, device="cuda", dtype=torch.int32)
+    h, pre = ffn.gated_linear_forward(x, wt)
+    for fn, args in ((ffn.gated_linear, (x, wt)), (ffn.gated_linear_forward, (x, wt)), (ffn.gated_linear_backward, (h, pre, x, wt)),
+                     (lambda *t: torch.ops.fp4ar.gated_linear(*t, 0), (x, wt)), (lambda *t: torch.ops.fp4ar.gated_linear_pre(*t, 0), (x, wt)),
+                     (lambda *t: torch.ops.fp4ar.gated_linear_backward(*t, 0, True, True), (h, pre, x, wt)),
+                     (lambda *t: AD.linear_adapters(t[0], t[1], ids, t[2], t[3]), (x, wt, a, b)),
+                     (lambda *t: torch.ops.fp4ar.linear_adapters(t[0], t[1], ids, t[2], t[3], None), (x, wt, a, b))):
+        fn(*args)
+        for i in range(len(args)):
+            with forward_ad.dual_level():
+                dual = list(args)
+                dual[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(RuntimeError, match="has no forward-mode derivative"):
+                    fn(*dual)
+    g = x.clone().requires_grad_()
+    for gated in (ffn.gated_linear, lambda p, q: torch.ops.fp4ar.gated_linear(p, q, 0)):      # forward over reverse
+        with forward_ad.dual_level(), pytest.raises(RuntimeError):
+            torch.autograd.grad(gated(g, wt), g, forward_ad.make_dual(h, h))
