@@ -99,6 +99,12 @@ inline void ok(int rc, const char* what) {
   if (rc != FP4AR_OK) raise_rc(rc, what);
 }
 
+// Kernels write behind autograd's back: who has saved a tensor for a backward pass learns of it by the version.  (A tensor made under
+// inference mode has none and cannot have been saved.)
+inline void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // ---- one function per op: used by the Python entry points (GIL released) and by torch.ops ----
 std::tuple<Tensor, Tensor> op_encode(const Tensor& x) {
   require(x, at::kBFloat16, kHidden, "x");
@@ -283,11 +289,13 @@ std::tuple<Tensor, Tensor> op_gated_linear(const Tensor& x, const Tensor& wt, in
     require_apart(out, wt, "wt");
   }
   const c10::cuda::CUDAGuard guard(dev);
-  if (!out.defined()) out = new_empty({s.M, s.F}, at::kBFloat16, dev);
+  const bool given = out.defined();
+  if (!given) out = new_empty({s.M, s.F}, at::kBFloat16, dev);
   Tensor pre;
   if (want_pre) pre = new_empty({s.M, 2 * s.F}, at::kFloat, dev);
   ok(api.gated_linear(x.data_ptr(), wt.data_ptr(), (int)s.M, (int)s.F, (int)s.K, (int)act, out.mutable_data_ptr(),
                       want_pre ? pre.mutable_data_ptr() : nullptr, stream_of(dev)), "fp4ar_gated_linear");
+  if (given) written(out);
   return {std::move(out), std::move(pre)};
 }
 
@@ -385,11 +393,13 @@ Tensor op_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, 
     if (scales.defined()) require_apart(out, scales, "scales");
   }
   const c10::cuda::CUDAGuard guard(dev);
-  if (!out.defined()) out = new_empty({M, Nn}, at::kBFloat16, dev);
+  const bool given = out.defined();
+  if (!given) out = new_empty({M, Nn}, at::kBFloat16, dev);
   Tensor ws = new_empty({(int64_t)api.adapters_workspace((int)M, (int)R, (int)n)}, at::kByte, dev);
   ok(api.linear_adapters(x.data_ptr(), wt.data_ptr(), (const int*)ids.data_ptr(), a.data_ptr(), b.data_ptr(),
                          scales.defined() ? (const float*)scales.data_ptr() : nullptr, (int)M, (int)Nn, (int)K, (int)R, (int)n,
                          ws.mutable_data_ptr(), out.mutable_data_ptr(), stream_of(dev)), "fp4ar_linear_adapters");
+  if (given) written(out);
   return out;
 }
 
