@@ -258,6 +258,14 @@ void require_apart(const Tensor& out, const Tensor& in, const char* name) {
 // Rows and columns as the C interface takes them: 32-bit, with room for a tile.
 void require_size(int64_t n, const char* name) { TORCH_CHECK_VALUE(n <= 0x7fff0000, name, " is too large: ", n); }
 
+bool recording(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+// Values with a gradient of their own are not written over: it would go on to whoever made them.
+void require_no_history(const Tensor& out) { TORCH_CHECK_VALUE(!recording({&out}), "out must not require a gradient"); }
 // A tangent that a kernel does not see would be lost: torch takes a result without one as constant.
 void require_no_tangent(std::initializer_list<const Tensor*> ts, const char* op) {
   for (const Tensor* t : ts)
@@ -281,6 +289,7 @@ struct GatedShape {
 
 std::tuple<Tensor, Tensor> op_gated_linear(const Tensor& x, const Tensor& wt, int64_t act, bool want_pre, Tensor out) {
   require_no_tangent({&x, &wt, &out}, "gated_linear");
+  require_no_history(out);
   const GatedShape s(x, wt, act);
   const c10::Device dev = x.device();
   if (out.defined()) {
@@ -345,12 +354,6 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     return out;
   }
 };
-bool recording(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : ts)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
 // h, recorded where autograd records
 Tensor op_gated_linear_auto(const Tensor& x, const Tensor& wt, int64_t act, Tensor out) {
   if (!recording({&x, &wt})) return std::get<0>(op_gated_linear(x, wt, act, false, std::move(out)));
@@ -364,6 +367,7 @@ void require_no_recording(std::initializer_list<const Tensor*> ts) {
 }
 Tensor op_linear_adapters(const Tensor& x, const Tensor& wt, const Tensor& ids, const Tensor& a, const Tensor& b, const Tensor& scales, Tensor out) {
   require_no_tangent({&x, &wt, &a, &b, &scales, &out}, "linear_adapters");
+  require_no_history(out);
   TORCH_CHECK_VALUE(x.dim() == 2, "x must have shape [rows, K], got ", shape_text(x));
   TORCH_CHECK_VALUE(wt.dim() == 2 && wt.size(1) == x.size(1), "wt must have shape [N, ", x.size(1), "], got ", shape_text(wt));
   const int64_t M = x.size(0), K = x.size(1), Nn = wt.size(0);

@@ -146,3 +146,20 @@ def test_the_custom_ops_have_no_forward_mode(ops):
     g = x.clone().requires_grad_()
     with pytest.raises(RuntimeError):
         _forward_mode(lambda d: torch.autograd.grad(ops.gated_linear(g, wt, 0), g, d), (h,), 0)
+
+
+def test_an_out_with_a_history_is_refused(ops):
+    """Its gradient would go on to whoever made the values that the call writes over."""
+    from fp4_all_reduce_b200.ops import adapters, ffn
+
+    x, wt = torch.zeros(5, 16, dtype=torch.bfloat16), torch.zeros(48, 16, dtype=torch.bfloat16)
+    t = list(_adapter_tensors(lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype)).values())
+    for fn, args, out in ((ffn.gated_linear, (x, wt), torch.zeros(5, 24, dtype=torch.bfloat16)),
+                          (ffn.gated_linear_forward, (x, wt), torch.zeros(5, 24, dtype=torch.bfloat16)),
+                          (adapters.linear_adapters, t, torch.zeros(5, 48, dtype=torch.bfloat16))):
+        leaf = out.requires_grad_()
+        for bad in (leaf, leaf * 2):
+            with pytest.raises(ValueError, match="out must not require a gradient"):
+                fn(*args, out=bad)
+            with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):       # nothing is recorded: taken as any other
+                fn(*args, out=bad)
