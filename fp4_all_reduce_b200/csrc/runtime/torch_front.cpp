@@ -208,12 +208,15 @@ std::tuple<Tensor, Tensor> op_norm(const Tensor& x, const Tensor& residual, cons
                       "out must be contiguous, on ", dev, " and hold ", bytes, " bytes");
   }
   const c10::cuda::CUDAGuard guard(dev);
+  const bool given = out.defined();
   Tensor res_out = inplace ? residual : new_empty(residual.sizes(), at::kBFloat16, dev);
-  if (!out.defined()) out = new_empty({rows, cols}, bf16 ? at::kBFloat16 : at::kByte, dev);
+  if (!given) out = new_empty({rows, cols}, bf16 ? at::kBFloat16 : at::kByte, dev);
   void* op = out.mutable_data_ptr();
   ok(api.add_rmsnorm(x.data_ptr(), residual.data_ptr(), res_out.mutable_data_ptr(), weight.data_ptr(), (float)eps, (float)weight_bias,
                      (int)epilogue, (float)qscale, bf16 ? op : nullptr, bf16 ? nullptr : op, (int)rows, stream_of(dev)),
      "fp4ar_add_rmsnorm");
+  if (given) written(out);
+  if (inplace) written(res_out);
   return {std::move(out), std::move(res_out)};
 }
 
@@ -228,7 +231,8 @@ std::tuple<Tensor, Tensor> op_gemm(const Tensor& x, const Tensor& wt, double gs,
   require_on(wt, dev, "wt");
   const c10::cuda::CUDAGuard guard(dev);
   const int64_t qb = Nn / 2 + Nn / 16;
-  if (!q.defined()) {
+  const bool given = q.defined();
+  if (!given) {
     q = new_empty({M, qb}, at::kByte, dev);
   } else {
     TORCH_CHECK_VALUE(layout_ok(q, at::kByte, qb) && q.size(0) == M && q.device() == dev,
@@ -238,6 +242,7 @@ std::tuple<Tensor, Tensor> op_gemm(const Tensor& x, const Tensor& wt, double gs,
   if (want_acc) acc = new_empty({M, Nn}, at::kFloat, dev);
   ok(api.gemm(nullptr, 0, x.data_ptr(), wt.data_ptr(), (int)M, (int)Nn, (int)K, (float)gs, q.mutable_data_ptr(),
               want_acc ? (float*)acc.mutable_data_ptr() : nullptr, stream_of(dev)), "fp4ar_gemm_nvfp4");
+  if (given) written(q);
   return {std::move(q), std::move(acc)};
 }
 
@@ -706,6 +711,7 @@ PyObject* ctx_all_reduce(PyObject* self, PyObject* const* p, Py_ssize_t n) {
   }
   a.out = out.mutable_data_ptr();
   launched(launch(c, a));
+  if (p[1] != Py_None) written(out);
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -739,6 +745,8 @@ PyObject* ctx_block(PyObject* self, PyObject* const* p, Py_ssize_t n) {
   a.res_out = res_out->mutable_data_ptr();
   a.weight = w->data_ptr();
   launched(launch(c, a));
+  if (p[9] != Py_None) written(out);
+  written(*res_out);
   return wrap2(std::move(out), *res_out);
   END_HANDLE_TH_ERRORS
 }

@@ -30,6 +30,14 @@ def _req_layout(t: torch.Tensor, dtype, cols: int | None, name: str) -> torch.Te
     return t
 
 
+def _written(*tensors: torch.Tensor | None) -> None:
+    """Kernels write behind autograd's back: whoever has saved a tensor for a backward pass learns of it by the version.  (A
+    tensor made under inference mode has none and cannot have been saved.)"""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def encode(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """BF16 [rows, 6144] -> (NVFP4 rows [rows, 3456] uint8: 3072 value bytes then 384 scale bytes,
     FP32 row scales [rows])."""

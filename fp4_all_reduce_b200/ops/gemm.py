@@ -16,6 +16,7 @@ from typing import Optional, Sequence
 import torch
 
 from .. import _native as N
+from .codec import _written
 
 
 def _stream() -> C.c_void_p:
@@ -68,6 +69,7 @@ def gemm_push(ctx, x: torch.Tensor, wt: torch.Tensor, gs_self: float, *, two_sho
         N.check(N.cuda().fp4ar_gemm_nvfp4(C.byref(view), 1 if two_shot else 0, x.data_ptr(), wt.data_ptr(), M, Nn, K,
                                           C.c_float(gs_self), local_q.data_ptr() if local_q is not None else None, None,
                                           _stream()), "fp4ar_gemm_nvfp4(push)")
+    _written(local_q)
 
 
 def gemm_all_reduce_add_rms_norm(ctx, x: torch.Tensor, wt: torch.Tensor, gs: Sequence[float], residual: torch.Tensor,
@@ -98,6 +100,7 @@ def gemm_all_reduce_add_rms_norm(ctx, x: torch.Tensor, wt: torch.Tensor, gs: Seq
     ctx.launch(make_args(x=None, out=o, rows=M, input=N.IN_PUSHED, gs=list(gs), epilogue=epilogue, res_in=residual,
                          res_out=residual, weight=weight, eps=eps, weight_bias=weight_bias, outq=q, qscale=qscale,
                          algo=N.ALGO_TWOSHOT if two_shot else N.ALGO_ONESHOT))
+    _written(out, residual)
     return (o if o is not None else q), residual
 
 

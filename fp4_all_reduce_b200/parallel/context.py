@@ -251,13 +251,17 @@ class Fp4ArContext(_Base):
             y = self._front.all_reduce(x, out, gs, algo, mode, teams)
             if y is not None:
                 return y
+        from ..ops.codec import _written
+
         kind = self._check_input(x, gs)
         rows = x.shape[0]
+        given = out
         if out is None:
             out = torch.empty(rows, N.HIDDEN, dtype=torch.bfloat16, device=x.device)
         else:
             self._check_like(out, torch.bfloat16, rows, N.HIDDEN, "out")
         self.launch(make_args(x=x, out=out, rows=rows, input=kind, gs=gs, algo=algo, mode=mode, teams=teams))
+        _written(given)
         return out
 
     def all_reduce_add_rms_norm(self, x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, *,
@@ -269,6 +273,8 @@ class Fp4ArContext(_Base):
             y = self._front.block(x, residual, weight, eps, weight_bias, epilogue, qscale, gs, algo, out, residual_out, mode, teams)
             if y is not None:
                 return y
+        from ..ops.codec import _written
+
         kind = self._check_input(x, gs)
         rows = x.shape[0]
         if epilogue not in (N.EPI_NORM_BF16, N.EPI_NORM_NVFP4, N.EPI_NORM_MXFP8):
@@ -293,6 +299,7 @@ class Fp4ArContext(_Base):
         self.launch(make_args(x=x, out=o, rows=rows, input=kind, gs=gs, algo=algo, epilogue=epilogue, res_in=residual,
                               res_out=res_out, weight=weight, eps=eps, weight_bias=weight_bias, outq=q, qscale=qscale,
                               mode=mode, teams=teams))
+        _written(out, res_out)
         return (o if o is not None else q), res_out
 
 
