@@ -303,6 +303,7 @@ gemm_nvfp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         bool ok = lane == 0 ? gemm_flag_wait(flag, 0u, gw, 5) : true;
         ok = __all_sync(0xffffffffu, ok) && __all_sync(0xffffffffu, gemm_wait(acc_full + a, (tile_i >> 1) & 1u, gw, 4));
         if (!ok) break;
+        __syncwarp();                                      // what lane 0 has acquired is ordered for the others too (a vote orders no memory)
         tc_fence_after();
         float v[2][32];
         tmem_ld32_issue(tbase, v[0]);
@@ -333,6 +334,7 @@ gemm_nvfp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         // written about one kernel duration ago; fetched while the last K blocks of this tile are still running
         bool ok = lane == 0 ? gemm_flag_wait(fix_flag, 1u, gw, 6) : true;
         if (!__all_sync(0xffffffffu, ok)) break;
+        __syncwarp();                                      // as above
         load_partial(0, pv[0]);
       }
       // warp-uniform verdict: the tcgen05.ld below is a warp-wide instruction

@@ -519,6 +519,7 @@ pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Para
       if (sg.kind == kFinish)
         for (int j = 1 + lane; j <= sg.others; j += 32) good = good && gemm_flag_wait(flag + 2 * kSplitFlags * j, 1u, gw, 6);
       if (!__all_sync(0xffffffffu, good)) break;
+      __syncwarp();                                        // what one lane has acquired is ordered for the others too (a vote orders no memory)
       if (sg.kind == kFinish && mine) load_shares(0);      // in flight while the last K blocks run
       if (!__all_sync(0xffffffffu, gemm_wait(acc_full + a, (tile_i >> 1) & 1u, gw, 4))) break;
       tc_fence_after();
