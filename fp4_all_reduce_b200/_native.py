@@ -146,6 +146,8 @@ def cuda() -> C.CDLL:
     lib.fp4ar_gated_backward.restype = C.c_int
     lib.fp4ar_adapters_workspace.argtypes = [C.c_int, C.c_int, C.c_int]
     lib.fp4ar_adapters_workspace.restype = C.c_size_t
+    lib.fp4ar_adapters_few_rows.argtypes = [C.c_int, C.c_int]
+    lib.fp4ar_adapters_few_rows.restype = C.c_int
     lib.fp4ar_linear_adapters.argtypes = [vp, vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp]
     lib.fp4ar_linear_adapters.restype = C.c_int
     lib.fp4ar_layer_plan.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, ip, ip, C.c_int]

@@ -34,6 +34,9 @@ size_t fp4ar_adapters_workspace(int M, int R, int adapters);
 int fp4ar_linear_adapters(const void* x, const void* wt, const int* ids, const void* a, const void* b, const float* scales, int M, int N,
                           int K, int R, int adapters, void* workspace, void* y, fp4ar_stream stream);
 
+/* Which kernel takes a call of fp4ar_linear_adapters (host only): 1 the one for few rows, 0 tiles of 256 rows, -1 for bad arguments. */
+int fp4ar_adapters_few_rows(int M, int adapters);
+
 /* How these products share their work (host only): `tiles` output tiles of `kblocks` K blocks over `units` CTA pairs.  *used: units that
  * work.  With `segments` the work of `unit` as (tile, first K block, K blocks, kind: 0 whole, 1 leaves a partial, 2 finishes the
  * tile, units that leave partials for it); returns the number of segments (also beyond max_segments), -1 for bad arguments. */

@@ -369,6 +369,11 @@ extern "C" size_t fp4ar_adapters_workspace(int M, int R, int adapters) {
   return Workspace(nullptr, M, R).bytes;
 }
 
+extern "C" int fp4ar_adapters_few_rows(int M, int adapters) {
+  if (M < 0 || adapters < 1) return -1;
+  return few_rows(M, adapters) ? 1 : 0;
+}
+
 extern "C" int fp4ar_linear_adapters(const void* x, const void* wt, const int* ids, const void* a, const void* b, const float* scales, int M,
                                      int N, int K, int R, int adapters, void* workspace, void* y, fp4ar_stream stream_) {
   if (!adapters_shape_ok(M, N, K, R, adapters)) return FP4AR_ERR_ARGUMENT;
