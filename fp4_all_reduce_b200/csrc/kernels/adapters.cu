@@ -345,11 +345,15 @@ __global__ void __launch_bounds__(256, 3) few_low_rank_kernel(const __nv_bfloat1
   }
 }
 
-// Which of the two products takes a call.  A tile of 256 rows pays 1.2 us and more for every adapter in it, the few-row kernel nothing,
-// but it reads W once for every 128 rows and B once for every row.  N = 6144, K = 2048, rank 16, us, few-row kernel / tiles: 128 rows
-// of 4 adapters 19 / 28; 200 rows of 4: 23 / 27, of 16: 24 / 45, of 64: 24 / 128; 512 rows of 8: 35 / 28, of 64: 37 / 130.  Rank 64,
-// K = 8192: 256 rows of 8: 97 / 72, of 64: 103 / 427.  How many adapters a tile has is known on the device alone, so the pool's
-// size stands in for it.
+// Which of the two products takes a call.  For every adapter in a tile of 256 rows a call in tiles pays about 1.5 us at rank 16, K = 2048, and
+// 5 - 6 at rank 64, K = 8192 (V's passes over x among them), the few-row kernel next to nothing, but it reads W once for every 128 rows
+// and B once for every row.  N = 6144, us, few-row kernel / tiles.  K = 2048, rank 16: 200 rows of 4 adapters 24 / 22, of 8: 25 / 27, of 12: 25 / 33; 300 rows of 8: 28 / 27, of 12: 28 / 33,
+// of 18: 28 / 43; 512 rows of 8: 38 / 27, of 16: 38 / 39, of 20: 38 / 47, of 31: 38 / 62, of 64: 37 / 130.  K = 8192, rank 64: 256 rows of
+// 8: 95 / 77, of 15: 96 / 116, of 64: 103 / 427; 512 rows of 16: 158 / 106, of 31: 158 / 183.
+// The limit of M / 16 adapters is thus too high, by up to twice at rank 16 (the two cross at 7 of 200, 9 of 300 and 15 of 512 rows), by a
+// fifth to a half at rank 64 (11 of 256, 26 of 512): just below it a call takes up to 1.6 times the other kernel's time.  How many
+// adapters a tile has is known on the device alone, so the pool's size stands in for it.  Beyond 512 rows only tiles take a call: 1024
+// rows of 1, 8 and 64 adapters 30, 48 and 198 us at rank 16, 35, 71 and 443 at rank 64 (K = 2048); 4096 rows 85, 129, 506 and 94, 176, 1113.
 static bool few_rows(int M, int adapters) { return M <= kNarrowRows || (M <= 512 && 16LL * adapters >= M); }
 
 }  // namespace layer

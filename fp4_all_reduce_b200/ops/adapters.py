@@ -9,7 +9,8 @@ parallelism every rank has its K columns of `wt` and `a` and all of `b`; y is it
 `ctx.all_reduce_add_rms_norm` (N = 6144 there, any multiple of 8 here).
 
 BF16 tensors, contiguous, starting on 16-byte boundaries; K, N and R are multiples of 8, R is at most 128.  All sums are FP32; x a.T is
-not rounded below 16 bits of mantissa before it meets b, and y is rounded once.  Runs on the current stream; forward only.
+not rounded below 16 bits of mantissa before it meets b, and y is rounded once.  Runs on the current stream; forward only: a call that
+autograd would record and tangents of forward mode are refused, by `torch.ops.fp4ar.linear_adapters` as well.
 """
 from __future__ import annotations
 

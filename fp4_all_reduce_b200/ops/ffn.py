@@ -12,6 +12,9 @@ gradient, to be summed by `ctx.all_reduce`.
 BF16 tensors, contiguous, starting on 16-byte boundaries; K and F are multiples of 8, M is any row count.  Sums, the activation and
 the product are FP32, h is rounded once.  The backward pass hands the gradients of
 the projections to its matrix products in BF16.  Everything runs on the current stream.
+
+Second derivatives and forward mode are refused, by `torch.ops.fp4ar.gated_linear` as well.  A given `out` gets a new version, as
+after any in-place operation; where autograd records it must not require a gradient.
 """
 from __future__ import annotations
 
@@ -39,5 +42,5 @@ def gated_linear_forward(x: torch.Tensor, wt: torch.Tensor, activation: int = N.
 def gated_linear_backward(dh: torch.Tensor, pre: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, activation: int = N.ACT_SILU, *,
                           need_dx: bool = True, need_dwt: bool = True) -> tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dwt) for the gradient dh of h, each None where it is not needed.  dh may have any strides and any place in
-    its storage."""
+    its storage.  Records no gradient."""
     return N.front().gated_backward(dh, pre, x, wt, activation, need_dx, need_dwt)
