@@ -21,6 +21,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 #include <torch/library.h>
@@ -350,10 +351,11 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     auto r = op_gated_backward(grads[0], saved[2], saved[0], saved[1], ctx->saved_data["activation"].toInt(), ctx->needs_input_grad(0),
                                ctx->needs_input_grad(1));
     torch::autograd::variable_list out{std::move(std::get<0>(r)), std::move(std::get<1>(r))};
-    if (at::GradMode::is_enabled()) {            // create_graph: the gradients cannot be differentiated again, and say so
-      for (Tensor& t : out)
-        if (t.defined()) t = t.detach().set_requires_grad(true);
-      out = (*std::make_shared<torch::autograd::DelayedError>("gated_linear cannot be differentiated twice", 2))(std::move(out));
+    if (at::GradMode::is_enabled()) {            // create_graph: the gradients cannot be differentiated again, and say so on every way back
+      auto refuses = std::make_shared<torch::autograd::Error>("gated_linear cannot be differentiated twice",
+                                                              torch::autograd::collect_next_edges(grads[0], saved[0], saved[1]));
+      for (const Tensor& t : out)
+        if (t.defined()) torch::autograd::set_history(t, refuses);
     }
     out.emplace_back();
     return out;

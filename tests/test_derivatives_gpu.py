@@ -68,3 +68,20 @@ def test_forward_mode_is_refused():
     for gated in (ffn.gated_linear, lambda p, q: torch.ops.fp4ar.gated_linear(p, q, 0)):      # forward over reverse
         with forward_ad.dual_level(), pytest.raises(RuntimeError):
             torch.autograd.grad(gated(g, wt), g, forward_ad.make_dual(h, h))
+
+
+@pytest.mark.parametrize("gated", [ffn.gated_linear, lambda x, wt: torch.ops.fp4ar.gated_linear(x, wt, 0)], ids=["ffn", "op"])
+def test_a_gradient_penalty_raises_where_only_some_gradients_are_asked_for(gated):
+    """autograd.grad and backward(inputs=...) run only what leads to the tensors they are given: the refusal stands on the way to every
+    input of the first backward pass."""
+    x, wt, dh = (t.requires_grad_() for t in (_bf16(4, 16), _bf16(48, 16, seed=1), _bf16(4, 24, seed=2)))
+    for wanted in ((x, wt), (x,), (wt,), (dh,)):
+        for first in (x, wt):
+            h = gated(x, wt)
+            (g,) = torch.autograd.grad(h, first, dh, create_graph=True)
+            with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+                torch.autograd.grad(h.sum() + g.square().sum(), wanted, allow_unused=True)
+            h = gated(x, wt)
+            (g,) = torch.autograd.grad(h, first, dh, create_graph=True)
+            with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+                (h.sum() + g.square().sum()).backward(inputs=list(wanted))
