@@ -443,6 +443,27 @@ Tensor lib_linear_adapters_autograd(c10::DispatchKeySet keys, const Tensor& x, c
   const at::AutoDispatchBelowAutograd below;
   return op.redispatch(keys & c10::after_autograd_keyset, x, wt, ids, a, b, scales);
 }
+// Autograd kernel of the two parts of the backward pass: they can be recorded (a gradient taken with create_graph=True, or a call of their
+// own), and whoever differentiates them hears that their derivatives do not exist.  Without it torch's fallback would leave those
+// out of the sums with no more than a warning.  (In Python it took 7 us of host time a call.)
+void lib_refuse_gradients(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  torch::autograd::edge_list edges;
+  if (at::GradMode::is_enabled()) {
+    for (size_t n = op.schema().arguments().size(), i = stack->size() - n; i < stack->size(); i++)
+      if ((*stack)[i].isTensor() && (*stack)[i].toTensor().requires_grad())
+        edges.push_back(torch::autograd::impl::gradient_edge((*stack)[i].toTensor()));
+  }
+  {
+    const at::AutoDispatchBelowAutograd below;
+    op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
+  }
+  if (edges.empty()) return;
+  const bool forward = op.schema().name() == "fp4ar::gated_linear_pre";
+  auto refuses = std::make_shared<torch::autograd::Error>(forward ? "gated_linear_pre records no gradient: differentiate gated_linear"
+                                                                  : "gated_linear cannot be differentiated twice", std::move(edges));
+  for (size_t n = op.schema().returns().size(), i = stack->size() - n; i < stack->size(); i++) torch::autograd::set_history((*stack)[i].toTensor(), refuses);
+}
+
 // Between autograd and the kernels of any device, for the ops above: no tangent gets past here.
 void lib_refuse_tangents(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
   for (size_t n = op.schema().arguments().size(), i = stack->size() - n; i < stack->size(); i++)
@@ -814,7 +835,10 @@ TORCH_LIBRARY_IMPL(fp4ar, ADInplaceOrView, m) {
   for (const char* op : {"gated_linear", "gated_linear_pre", "gated_linear_backward", "linear_adapters"})
     m.impl(op, torch::CppFunction::makeFromBoxedFunction<&lib_refuse_tangents>());
 }
-TORCH_LIBRARY_IMPL(fp4ar, Autograd, m) { m.impl("linear_adapters", TORCH_FN(lib_linear_adapters_autograd)); }
+TORCH_LIBRARY_IMPL(fp4ar, Autograd, m) {
+  m.impl("linear_adapters", TORCH_FN(lib_linear_adapters_autograd));
+  for (const char* op : {"gated_linear_pre", "gated_linear_backward"}) m.impl(op, torch::CppFunction::makeFromBoxedFunction<&lib_refuse_gradients>());
+}
 
 PyMODINIT_FUNC PyInit__fp4ar_front() {
   ctx_type.tp_name = "_fp4ar_front.Context";

@@ -214,16 +214,3 @@ def _gated_grad(ctx, dh):
 
 
 torch.library.register_autograd("fp4ar::gated_linear", _gated_grad, setup_context=_gated_setup)
-
-
-# The parts of the backward pass can be recorded (a gradient taken with create_graph=True, or a call of their own), but their
-# derivatives do not exist; without a formula torch's fallback would leave them out of the sums with no more than a warning.
-def _refuses(message):
-    def backward(ctx, *grads):
-        raise RuntimeError(message)
-
-    return backward
-
-
-torch.library.register_autograd("fp4ar::gated_linear_pre", _refuses("gated_linear_pre records no gradient: differentiate gated_linear"))
-torch.library.register_autograd("fp4ar::gated_linear_backward", _refuses("gated_linear cannot be differentiated twice"))
